@@ -1,0 +1,329 @@
+"""Copied rows, steered logits and log-probabilities on the GPU, against copies and loops in 64 bits."""
+import numpy as np
+import pytest
+import torch
+
+from steering_cases import adjusted, history_tensors, log_probs_in_64, random_rules
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from transformers_neuronx_amd.kernels import make_ops
+    return make_ops("hip", torch.float32, "cuda:0")
+
+
+# ---------------------------------------------------------------- rows
+
+def _pages(shapes, dtype, pad, seed, rows=13):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    out = []
+    for shape in shapes:
+        count = int(np.prod(shape))
+        whole = torch.empty(rows, count + pad, device="cuda", dtype=dtype)
+        whole.copy_(torch.randn(whole.shape, generator=g, device="cuda") * 8)
+        out.append(whole[:, :count].view(rows, *shape))
+    return out
+
+
+def _copied(tensors, axes, sources, targets, tokens):
+    out = [t.clone() for t in tensors]
+    for i, (s, d) in enumerate(zip(sources, targets)):
+        for t, axis in zip(out, axes):
+            n = t.shape[axis] if axis is not None and tokens is None else None if axis is None else tokens[i]
+            if axis is None:
+                t[d].copy_(t[s])
+            else:
+                t[d].narrow(axis - 1, 0, n).copy_(t[s].narrow(axis - 1, 0, n))
+    return out
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32, torch.uint8])
+@pytest.mark.parametrize("heads, page, size, pad", [(1, 16, 2, 0), (2, 16, 8, 16), (3, 64, 80, 192), (5, 48, 33, 8), (1, 16, 1, 1), (4, 32, 128, 3)])
+def test_copied_rows(ops, dtype, heads, page, size, pad):
+    tensors = _pages([(heads, page, size), (heads, size, page), (7,), (heads, page)], dtype, pad, seed=page + size)
+    axes = [2, 3, None, 2]
+    rows = ops.row_set(tensors, axes)
+    for sources, targets, tokens in (([3], [0], [page]), ([5, 5, 5, 1], [12, 0, 2, 4], [1, 1, 1, page - 1]),
+                                     ([0, 1, 1, 2], [8, 9, 10, 11], [0, 3, 5, 7]), ([9, 8, 7], [6, 1, 0], None)):
+        want = _copied(tensors, axes, sources, targets, tokens)
+        ops.copy_rows(rows, sources, targets, tokens)
+        assert all(torch.equal(a, b) for a, b in zip(tensors, want)), (sources, targets, tokens)
+
+
+def test_rows_leave_what_lies_between_them(ops):
+    whole = torch.arange(8 * 40, device="cuda", dtype=torch.float32).view(8, 40)
+    before = whole.clone()
+    ops.copy_rows(ops.row_set([whole[:, 4:37].view(8, 3, 11)], [1]), [0, 6], [3, 7], [2, 3])
+    before[3, 4:26], before[7, 4:37] = before[0, 4:26], before[6, 4:37]
+    assert torch.equal(whole, before)
+
+
+def test_rows_of_many_sources_and_targets(ops):
+    t = torch.randn(2000, 24, device="cuda")
+    order = np.random.default_rng(1).permutation(2000)
+    sources, targets = np.repeat(order[:150], 10), order[150:1650]
+    want = t.clone()
+    want[torch.from_numpy(targets).cuda()] = t[torch.from_numpy(sources).cuda()]
+    ops.copy_rows(ops.row_set([t]), sources, targets)
+    assert torch.equal(t, want)
+
+
+def test_rows_beyond_four_gigabytes(ops):
+    """Row 5 of a tensor of rows 1 GB apart begins beyond 32 bits of bytes."""
+    whole = torch.zeros(6, 1 << 28, device="cuda", dtype=torch.float32)
+    t = whole[:, :1000]
+    t[5] = torch.arange(1000, device="cuda")
+    ops.copy_rows(ops.row_set([t]), [5], [4])
+    assert torch.equal(t[4], t[5]) and not t[:4].any()
+
+
+def test_rows_to_tensors_of_another_size(ops):
+    a, b = _pages([(2, 16, 24)], torch.bfloat16, 16, 3, rows=5)[0], _pages([(2, 16, 24)], torch.bfloat16, 48, 4, rows=11)[0]
+    want = b.clone()
+    want[10], want[0, :, :7] = a[4], a[1, :, :7]
+    ops.copy_rows(ops.row_set([a], [2], targets=[b]), [4, 1], [10, 0], [16, 7])
+    assert torch.equal(b, want)
+
+
+# ---------------------------------------------------------------- adjusted logits
+
+def _adjust(ops, case, logits=None):
+    from transformers_neuronx_amd.kernels.steering import TokenHistory
+    e, u = history_tensors(case, "cuda")
+    logits = torch.from_numpy(case["logits"]).cuda() if logits is None else logits
+    rules = ops.logit_rules(case["vocab"], **case["rules"])
+    last, masks = torch.from_numpy(case["last"]).cuda(), torch.from_numpy(case["masks"]).cuda()
+    return logits, rules, TokenHistory(e, u), last, masks
+
+
+def _check_adjusted(case, logits, history):
+    want, entries, used = adjusted(case)
+    assert np.array_equal(history.entries.cpu().numpy(), entries) and np.array_equal(history.used.cpu().numpy(), used)
+    got = logits.cpu().numpy()
+    assert np.array_equal(np.isneginf(got), np.isneginf(want)) and np.array_equal(np.isnan(got), np.isnan(want))
+    assert np.array_equal(np.isposinf(got), np.isposinf(want))
+    fine = np.isfinite(want)
+    # a quotient or product, a product and a sum, a difference, a sum: five roundings of half a step of what is added
+    assert (np.abs(got[fine] - want[fine]) <= 5 * 2.0 ** -24 * case["scale"][fine]).all()
+
+
+@pytest.mark.parametrize("rows, vocab, seen, biases, allowed", [
+    (1, 1, 1, 1, -1.0), (1, 1, 1, 1, 0.0), (2, 7, 7, 7, 0.5), (3, 31, 31, 10, 0.0), (4, 32, 5, 0, 1.0), (4, 33, 33, 33, 0.9),
+    (5, 1000, 0, 0, -1.0), (5, 1003, 400, 30, 0.001), (9, 4097, 3000, 700, 0.5), (3, 32001, 2500, 300, 0.98), (2, 50272, 1500, 300, 0.002),
+    (64, 513, 100, 10, 0.5)])
+def test_adjusted_logits(ops, rows, vocab, seen, biases, allowed):
+    case = random_rules(rows, vocab, seen, biases, allowed, seed=rows * 7 + vocab)
+    logits, rules, history, last, masks = _adjust(ops, case)
+    out = ops.adjust_logits(logits, rules, history, last, masks)
+    assert out is logits
+    _check_adjusted(case, logits, history)
+
+
+def test_rows_that_begin_anywhere(ops):
+    """Logits that are a part of a larger tensor, beginning 4 bytes behind a boundary of 16; what lies around them stays."""
+    case = random_rules(6, 1001, 300, 40, 0.5, seed=3)
+    whole = torch.full((6 * 1001 + 9,), 7.0, device="cuda")
+    part = whole[1:1 + 6 * 1001].view(6, 1001)
+    part.copy_(torch.from_numpy(case["logits"]))
+    logits, rules, history, last, masks = _adjust(ops, case, part)
+    ops.adjust_logits(logits, rules, history, last, masks)
+    _check_adjusted(case, logits, history)
+    assert whole[0] == 7 and (whole[1 + 6 * 1001:] == 7).all()
+
+
+def test_odd_values_under_rules(ops):
+    """Masked places become -inf whatever they were; a bias of -inf bars a token at +inf too; NaN elsewhere stays one."""
+    inf, nan = float("inf"), float("nan")
+    low = torch.finfo(torch.float32).min
+    logits = torch.tensor([[nan, inf, -inf, low, 1.0, inf, nan, -2.0]], device="cuda")
+    masks = torch.tensor([[0b11111000]], dtype=torch.int32, device="cuda")
+    ops.adjust_logits(logits, ops.logit_rules(8, biases=[{5: -inf, 4: 2.0, 7: -1.0}], mask_rows=[0]), masks=masks)
+    assert logits[0, :3].tolist() == [-inf] * 3 and logits[0, 3] == low and logits[0, 4] == 3 and logits[0, 5] == -inf
+    assert torch.isnan(logits[0, 6]) and logits[0, 7] == -3
+
+
+def test_a_full_history_and_tokens_of_no_vocabulary(ops):
+    """A history without room takes no further token; entries and tokens outside the vocabulary touch nothing."""
+    from transformers_neuronx_amd.kernels.steering import TokenHistory
+    entries = torch.tensor([[[0, 2], [1, 2]], [[50, 2], [-3, 2]]], dtype=torch.int32, device="cuda")
+    used = torch.tensor([2, 2], dtype=torch.int32, device="cuda")
+    logits = torch.ones(2, 4, device="cuda")
+    rules = ops.logit_rules(4, slots=[0, 1], presence=[0.5, 0.5])
+    ops.adjust_logits(logits, rules, TokenHistory(entries.clone(), used), torch.tensor([3, 99], dtype=torch.int32, device="cuda"))
+    assert logits.tolist() == [[0.5, 0.5, 1, 1], [1, 1, 1, 1]] and used.tolist() == [2, 2]
+
+
+def test_histories_over_steps_and_replays(ops):
+    """A step recorded and replayed enters each step's token and gives what the eager steps give."""
+    vocab, rows = 1500, 5
+    g = torch.Generator(device="cuda").manual_seed(2)
+    rng = np.random.default_rng(2)
+    prompts = [rng.integers(0, vocab, n).tolist() for n in (1, 40, 300, 0, 7)]
+    steps = [(torch.randn(rows, vocab, generator=g, device="cuda"), torch.randint(0, 60, (rows,), generator=g, device="cuda").to(torch.int32))
+             for _ in range(6)]
+    slots = [4, 0, 3, 1, 2]
+    rules = ops.logit_rules(vocab, slots=slots, repetition=[1.3] * rows, presence=[0.4] * rows, frequency=[0.2] * rows)
+
+    def start():
+        h, last = ops.token_history(rows, vocab), torch.full((rows,), 9, dtype=torch.int32, device="cuda")
+        ops.start_history(h, slots, prompts, last=last)
+        assert last.tolist() == [-1] * rows
+        return h, last
+    eager, (h, last) = [], start()
+    for x, chosen in steps:
+        eager.append(ops.adjust_logits(x.clone(), rules, h, last))
+        last.copy_(chosen)
+    want = h.entries.clone(), h.used.clone()
+    h, last = start()
+    static = steps[0][0].clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ops.adjust_logits(static, rules, h, last)
+    for (x, chosen), y in zip(steps, eager):
+        static.copy_(x)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(static, y)
+        last.copy_(chosen)
+    assert torch.equal(h.entries, want[0]) and torch.equal(h.used, want[1])
+    # and what the histories hold is what a list of the same tokens gives
+    from transformers_neuronx_amd.kernels.steering import TokenHistory
+    for i, s in enumerate(slots):
+        chosen = [int(c[s]) for _, c in steps[:-1]]
+        entries = TokenHistory.distinct(prompts[i], chosen)
+        assert h.used[s] == len(entries) and np.array_equal(h.entries[s, :len(entries)].cpu().numpy(), entries)
+
+
+# ---------------------------------------------------------------- log-probabilities
+
+def _check_log_probs(logits, tokens, top, got):
+    want, want_ids, want_best = log_probs_in_64(logits.cpu().numpy(), tokens.cpu().numpy(), top)
+    # A logit less the largest is rounded once (2^-24 of it), the logarithm of a sum to a few 2^-24 of itself and of the sum's own
+    # error: the sum of n terms in 32 bits is off by at most log2(n) + n / 256 roundings where threads add up their own terms first.
+    vocab = logits.shape[1]
+    steps = 8 + np.log2(vocab) + vocab / 256
+    for a, b in ((got[0], want), (got[2], want_best)) if top else ((got[0], want),):
+        a = a.cpu().numpy().astype(np.float64)
+        assert np.array_equal(np.isfinite(a), np.isfinite(b)) and np.array_equal(np.isneginf(a), np.isneginf(b))
+        fine = np.isfinite(b)
+        assert (np.abs(a[fine] - b[fine]) <= steps * 2.0 ** -24 * (1 + np.abs(b[fine]))).all()
+    if top:
+        assert np.array_equal(got[1].cpu().numpy(), want_ids)
+    else:
+        assert got[1] is None and got[2] is None
+
+
+@pytest.mark.parametrize("rows, vocab, top", [
+    (1, 1, 1), (1, 2, 2), (3, 31, 31), (2, 32, 32), (5, 63, 1), (4, 257, 20), (7, 1000, 0), (3, 1023, 5), (2, 1025, 32), (9, 4096, 3),
+    (1, 16384, 20), (2, 32001, 20), (1, 50272, 32), (33, 50272, 5), (300, 513, 2), (2, 70001, 9), (1, 200003, 32)])
+def test_log_probs(ops, rows, vocab, top):
+    g = torch.Generator(device="cuda").manual_seed(vocab + top)
+    logits = torch.randn(rows, vocab, generator=g, device="cuda") * 3
+    logits[:, vocab // 2] += 9
+    tokens = torch.randint(0, vocab, (rows,), generator=g, device="cuda").to(torch.int32)
+    _check_log_probs(logits, tokens, top, ops.log_probs(logits, tokens, top))
+
+
+@pytest.mark.parametrize("vocab", [5, 300, 5000, 50272])
+@pytest.mark.parametrize("how", ["equal", "few values", "rising", "falling", "barred", "blocks"])
+def test_log_probs_of_ties_and_orders(ops, how, vocab):
+    """Rows whose largest logits are many, alike, or all in one place."""
+    i = torch.arange(vocab, device="cuda", dtype=torch.float32)
+    row = {"equal": torch.zeros_like(i), "few values": (i * 7) % 3, "rising": i / vocab * 9, "falling": -i / vocab * 9,
+           "barred": torch.where(i % 97 == 3, i / vocab, torch.tensor(float("-inf"), device="cuda")),
+           "blocks": torch.where((i % 1024) < 4, 5 + i / vocab, -i / vocab)}[how]
+    logits = torch.stack([row, row.roll(1), -row])
+    tokens = torch.tensor([0, vocab // 2, vocab - 1], dtype=torch.int32, device="cuda")
+    top = min(20, vocab)
+    _check_log_probs(logits, tokens, top, ops.log_probs(logits, tokens, top))
+
+
+@pytest.mark.parametrize("vocab", [3, 40, 3000])
+def test_log_probs_of_rows_with_infinities(ops, vocab):
+    inf, nan = float("inf"), float("nan")
+    logits = torch.randn(7, vocab, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda")
+    logits[0] = -inf
+    logits[1, [0, vocab - 1]] = inf
+    logits[2, 0], logits[2, vocab - 1] = nan, -inf
+    logits[3] = nan
+    logits[4] = inf
+    logits[5, 1:] = -inf
+    logits[6, :2] = torch.finfo(torch.float32).min
+    tokens = torch.tensor([0, vocab - 1, 0, 1, 2, vocab, -1], dtype=torch.int32, device="cuda")
+    top = min(5, vocab)
+    _check_log_probs(logits, tokens, top, ops.log_probs(logits, tokens, top))
+
+
+def test_log_probs_of_a_part_and_in_a_graph(ops):
+    g = torch.Generator(device="cuda").manual_seed(4)
+    whole = torch.randn(4 * 999 + 3, generator=g, device="cuda")
+    logits = whole[3:].view(4, 999)
+    tokens = torch.randint(0, 999, (4,), generator=g, device="cuda").to(torch.int32)
+    want = ops.log_probs(logits, tokens, 7)
+    _check_log_probs(logits, tokens, 7, want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = ops.log_probs(logits, tokens, 7)
+    for k in range(3):
+        logits.copy_(torch.randn(4, 999, generator=g, device="cuda"))
+        graph.replay()
+        torch.cuda.synchronize()
+        eager = ops.log_probs(logits, tokens, 7)
+        assert all(torch.equal(a, b) for a, b in zip(got, eager))
+
+
+def test_on_another_stream(ops):
+    """Everything is launched on the current stream."""
+    case = random_rules(4, 3001, 500, 30, 0.5, seed=11)
+    side = torch.cuda.Stream()
+    t = torch.randn(6, 5, 64, device="cuda")
+    want = t.clone()
+    want[3] = want[1]
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        logits, rules, history, last, masks = _adjust(ops, case)
+        ops.adjust_logits(logits, rules, history, last, masks)
+        got = ops.log_probs(logits, last[:4].clamp(min=0), 3)
+        ops.copy_rows(ops.row_set([t]), [1], [3])
+    side.synchronize()
+    _check_adjusted(case, logits, history)
+    _check_log_probs(logits, last[:4].clamp(min=0), 3, got)
+    assert torch.equal(t, want)
+
+
+def test_refusals(ops):
+    from transformers_neuronx_amd.kernels.steering import TokenHistory
+    x = torch.zeros(2, 40, device="cuda")
+    tokens = torch.zeros(2, dtype=torch.int32, device="cuda")
+    history = ops.token_history(2, 8)
+    last = torch.zeros(2, dtype=torch.int32, device="cuda")
+    plain, kept, masked = ops.logit_rules(40, rows=2), ops.logit_rules(40, slots=[0, 2]), ops.logit_rules(40, mask_rows=[1, 0])
+    good = torch.zeros(2, 2, dtype=torch.int32, device="cuda")
+    for call in (lambda: ops.adjust_logits(x[:, :39], plain), lambda: ops.adjust_logits(x[:1], plain), lambda: ops.adjust_logits(x.cpu(), plain),
+                 lambda: ops.adjust_logits(x.t().contiguous().t(), plain), lambda: ops.adjust_logits(x, kept),
+                 lambda: ops.adjust_logits(x, kept, history, last), lambda: ops.adjust_logits(x, ops.logit_rules(40, slots=[0, 1]), history, last[:1]),
+                 lambda: ops.adjust_logits(x, masked), lambda: ops.adjust_logits(x, masked, masks=good[:1]),
+                 lambda: ops.adjust_logits(x, masked, masks=torch.zeros(2, 1, dtype=torch.int32, device="cuda")),
+                 lambda: ops.start_history(history, [0], [list(range(9))]), lambda: ops.start_history(history, [0, 0], [[1], [2]]),
+                 lambda: ops.start_history(history, [2], [[1]]), lambda: ops.start_history(history, [0], [[-1]]),
+                 lambda: ops.start_history(history, [0], [[1]], last=last[:1]), lambda: ops.start_history(history, [0], []),
+                 lambda: ops.log_probs(x, tokens[:1]), lambda: ops.log_probs(x, tokens, 33), lambda: ops.log_probs(x, tokens, -1),
+                 lambda: ops.log_probs(x[:, :3].contiguous(), tokens, 4), lambda: ops.log_probs(x.cpu(), tokens), lambda: ops.log_probs(x[0], tokens),
+                 lambda: ops.row_set([torch.zeros(3, 4)]), lambda: TokenHistory(torch.zeros(2, 8, 2), torch.zeros(2))):
+        with pytest.raises(ValueError):
+            call()
+    for call in (lambda: ops.adjust_logits(x.double(), plain), lambda: ops.log_probs(x.bfloat16(), tokens), lambda: ops.log_probs(x, tokens.long())):
+        with pytest.raises(TypeError):
+            call()
+    rows = ops.row_set([torch.zeros(3, 4, device="cuda")])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(RuntimeError, match="recorded"):
+            ops.copy_rows(rows, [0], [1])
+        with pytest.raises(RuntimeError, match="recorded"):
+            ops.logit_rules(40, rows=2)
+        x.add_(1)
+    assert ops.adjust_logits(x[:0], ops.logit_rules(40, rows=0)).shape == (0, 40)
+    assert ops.log_probs(x[:0], tokens[:0], 2)[1].shape == (0, 2)

@@ -14,6 +14,8 @@ import torch
 from . import LostStep, build
 from .attention_plan import QUERY_TILE
 from .memory_plan import MEMORY_CHUNK
+from .row_set import RowSet
+from .steering import LogitRules, TokenHistory, mask_words
 from .. import debug
 
 _F32, _BF16 = 0, 1
@@ -229,6 +231,15 @@ _SIGNATURES = {
     "layer": {
         "tnx_decode_layer_words": [_c_int, _c_int, _c_int, _c_int, _c_int],
         "tnx_decode_layers": [_c_void_p, _c_int, _c_void_p],
+    },
+    "rows": {
+        "tnx_copy_rows": [_c_void_p, _c_int, _c_void_p, _c_int, _c_ll, _c_void_p],
+    },
+    "steering": {
+        "tnx_start_history": [_c_void_p, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_void_p],
+        "tnx_adjust_logits": [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_int,
+                              _c_int, _c_void_p],
+        "tnx_log_probs": [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_void_p],
     },
     "probe": {
         "tnx_probe_stream_read": [_c_void_p, ctypes.c_size_t, _c_void_p, _c_int, _c_void_p],
@@ -2875,6 +2886,161 @@ class HipOps:
         self._call("sampling", "tnx_sample", _ptr(logits), _ptr(temperature), _ptr(top_k), _ptr(top_p), _ptr(seeds),
                    _ptr(counters), _ptr(min_keep), _ptr(out), m, logits.shape[1], _stream())
         return out
+
+    # ---------------------------------------------------------------- several answers to one prompt
+
+    def _on_this_device(self, device, what):
+        """Launches go to the current device's stream: what they work on lies there."""
+        if device.type != "cuda":
+            raise ValueError(f"{what} must be on the GPU")
+        if device.index != torch._C._cuda_getDevice():
+            raise ValueError(f"{what} on {device}, but the current device is cuda:{torch._C._cuda_getDevice()}")
+
+    def _from_host(self, flat, what):
+        """`send_ints` for what is made of the host's lists: not while a graph is recorded, whose replays would read what the
+        pinned memory holds by then."""
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError(f"{what} takes lists from the host and cannot be recorded into a graph")
+        return self.send_ints(flat)
+
+    def row_set(self, tensors, token_axes=None, targets=None) -> RowSet:
+        """See `RowSet`; what `copy_rows` works on."""
+        rows = RowSet(tensors, token_axes, targets)
+        self._on_this_device(rows.device, "rows")
+        rows.table = self._from_host(rows.words.reshape(-1).view(np.int32), "row_set")
+        return rows
+
+    def copy_rows(self, rows: RowSet, sources, targets, tokens=None) -> None:
+        """In every tensor of the set, row `targets[i]` becomes a copy of row `sources[i]`: of its first `tokens[i]` places where
+        the tensor counts tokens, or whole (`tokens` None, or a tensor without a token axis). What lies behind them stays as it
+        was. The rows are lists on the host; a source may be named several times, a target once and not as a source too."""
+        pairs = rows.pairs(sources, targets, tokens)
+        if len(pairs) == 0:
+            return
+        if rows.table is None:
+            raise ValueError("this set of rows was not made by row_set")
+        self._on_this_device(rows.device, "rows")
+        dev = self._from_host(pairs.reshape(-1), "copy_rows")
+        self._call("rows", "tnx_copy_rows", _ptr(rows.table), len(rows.tensors), _ptr(dev), len(pairs), rows.largest, _stream(),
+                   work=lambda: (f"{len(pairs)} rows", 2 * len(pairs) * rows.row_bytes, 0))
+
+    def token_history(self, slots: int, capacity: int) -> TokenHistory:
+        """Empty histories for `slots` sequences of at most `capacity` distinct tokens."""
+        return TokenHistory(torch.zeros(slots, capacity, 2, dtype=torch.int32, device=self.device),
+                            torch.zeros(slots, dtype=torch.int32, device=self.device))
+
+    def start_history(self, history: TokenHistory, slots, prompts, outputs=None, last=None) -> None:
+        """The histories of `slots` become those of these tokens: each sequence's prompt and what it has chosen since. `last`
+        (int32, one a slot): the slots' entries become -1, no token is to be entered there."""
+        if len(prompts) != len(slots) or (outputs is not None and len(outputs) != len(slots)):
+            raise ValueError(f"{len(slots)} slots, {len(prompts)} prompts, {len(outputs or prompts)} outputs")
+        if not len(slots):
+            return
+        if len(set(slots)) != len(slots):
+            raise ValueError("a slot is named twice")
+        if min(slots) < 0 or max(slots) >= history.slots:
+            raise ValueError(f"slot {min(slots) if min(slots) < 0 else max(slots)} is outside the {history.slots} there are")
+        lists = [TokenHistory.distinct(p, () if outputs is None else outputs[i]) for i, p in enumerate(prompts)]
+        longest = max(len(e) for e in lists)
+        if longest > history.capacity:
+            raise ValueError(f"a sequence of {longest} distinct tokens, the history holds {history.capacity}")
+        if any(len(e) and e[:, 0].min() < 0 for e in lists):
+            raise ValueError("a token is below zero")
+        self._on_this_device(history.entries.device, "history")
+        if last is not None:
+            _want(last, "last", torch.int32)
+            if last.numel() < history.slots:
+                raise ValueError(f"last has {last.numel()} entries for {history.slots} slots")
+        heads, at = np.zeros((len(slots), 3), dtype=np.int32), 0
+        for i, (s, e) in enumerate(zip(slots, lists)):
+            heads[i] = s, at, len(e)
+            at += len(e)
+        room = -(-heads.size // 4) * 4                     # the pairs begin on 16 bytes
+        flat = np.zeros(room + 2 * at, dtype=np.int32)
+        flat[:heads.size] = heads.reshape(-1)
+        if at:
+            flat[room:] = np.concatenate(lists).reshape(-1)
+        dev = self._from_host(flat, "start_history")
+        self._call("steering", "tnx_start_history", _ptr(dev), len(slots), _ptr(dev[room:]), _ptr(history.entries), _ptr(history.used),
+                   _ptr(last), history.slots, history.capacity, _stream())
+
+    def logit_rules(self, vocab, rows=None, slots=None, repetition=None, presence=None, frequency=None, biases=None,
+                    mask_rows=None) -> LogitRules:
+        """See `LogitRules`; what `adjust_logits` goes by. `rows`: as many as the lists have, where one is given."""
+        if rows is None:
+            given = [len(v) for v in (slots, repetition, presence, frequency, biases, mask_rows) if v is not None]
+            if not given:
+                raise ValueError("logit_rules needs the number of rows, or a list with a value for each")
+            rows = given[0]
+        rules = LogitRules(int(vocab), rows, slots, repetition, presence, frequency, biases, mask_rows)
+        if rules.flat.size:
+            rules.device_words = self._from_host(rules.flat, "logit_rules")
+        return rules
+
+    def adjust_logits(self, logits, rules: LogitRules, history: Optional[TokenHistory] = None, last=None, masks=None):
+        """In place, row by row: `last[slot]` (int32; below zero: none) is entered into the row's history as chosen once more;
+        every token of the history is penalised, x / repetition where x > 0 and x * repetition elsewhere, less
+        frequency * times chosen, less presence if it was chosen; the row's biases are added; and tokens whose bit the row's mask
+        lacks become -inf, whatever they were. `masks`: int32 `[masks, mask_words(vocab)]`, bit t % 32 of word t // 32 for
+        token t (`pack_mask`). Returns the logits."""
+        _want(logits, "logits", torch.float32, (rules.rows, rules.vocab))
+        if rules.rows == 0:
+            return logits
+        if rules.device_words is None:
+            raise ValueError("these rules were not made by logit_rules")
+        self._on_this_device(logits.device, "logits")
+        if rules.device_words.device != logits.device:
+            raise ValueError("logits and rules lie on different devices")
+        if rules.most_slot >= 0:
+            if history is None or last is None:
+                raise ValueError("rows with a slot need the history, and the tokens chosen last")
+            _want(history.entries, "history", torch.int32)
+            _want(last, "last", torch.int32)
+            if history.entries.device != logits.device or last.device != logits.device:
+                raise ValueError("logits, history and last lie on different devices")
+            if rules.most_slot >= min(history.slots, last.numel()):
+                raise ValueError(f"slot {rules.most_slot} is outside the history's {history.slots} or the {last.numel()} of last")
+        else:
+            history = last = None
+        if rules.most_mask >= 0:
+            if masks is None:
+                raise ValueError("rows with a mask need the masks")
+            _want(masks, "masks", torch.int32)
+            if masks.dim() != 2 or masks.shape[1] != mask_words(rules.vocab) or masks.device != logits.device:
+                raise ValueError(f"masks are [masks, {mask_words(rules.vocab)}] beside the logits, got {tuple(masks.shape)} on {masks.device}")
+            if rules.most_mask >= masks.shape[0]:
+                raise ValueError(f"mask {rules.most_mask} is outside the {masks.shape[0]} there are")
+        else:
+            masks = None
+        heads, tokens, values = rules.pieces(rules.device_words)
+        self._call("steering", "tnx_adjust_logits", _ptr(logits), _ptr(heads), _ptr(tokens), _ptr(values),
+                   _ptr(history.entries) if history else None, _ptr(history.used) if history else None,
+                   history.capacity if history else 0, _ptr(last), _ptr(masks), rules.rows, rules.vocab, _stream())
+        return logits
+
+    MOST_TOP = 32         # alternatives that `log_probs` gives at most
+
+    def log_probs(self, logits, tokens, top=0):
+        """(float32 `[rows]`: the log-probability of each row's token; int32 `[rows, top]`: the row's largest logits' tokens, ties
+        to the lower id; float32 `[rows, top]`: their log-probabilities), the latter two None without `top`. Under a softmax over
+        the whole row; a NaN counts as -inf. A token outside the vocabulary has -inf, and so has every token of a row that is
+        -inf throughout; tokens at +inf share the whole among them."""
+        _want(logits, "logits", torch.float32)
+        if logits.dim() != 2:
+            raise ValueError(f"logits are [rows, vocab], got {tuple(logits.shape)}")
+        rows, vocab = logits.shape
+        _want(tokens, "tokens", torch.int32, (rows,))
+        if not 0 <= top <= min(self.MOST_TOP, vocab):
+            raise ValueError(f"top is 0 to {min(self.MOST_TOP, vocab)}, got {top}")
+        self._on_this_device(logits.device, "logits")
+        if tokens.device != logits.device:
+            raise ValueError("logits and tokens lie on different devices")
+        out = torch.empty(rows, dtype=torch.float32, device=logits.device)
+        ids = torch.empty(rows, top, dtype=torch.int32, device=logits.device) if top else None
+        best = torch.empty(rows, top, dtype=torch.float32, device=logits.device) if top else None
+        self._call("steering", "tnx_log_probs", _ptr(logits), _ptr(tokens), _ptr(out), _ptr(ids), _ptr(best), top, rows, vocab, _stream(),
+                   work=lambda: (f"{rows}x{vocab} top {top}", rows * (4 * vocab + 8 + 8 * top), 4.0 * rows * vocab))
+        return out, ids, best
 
     def synchronize(self):
         torch.cuda.synchronize(self.device)

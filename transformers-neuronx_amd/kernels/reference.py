@@ -11,6 +11,9 @@ from typing import Optional
 
 import torch
 
+from .row_set import RowSet
+from .steering import LogitRules, TokenHistory
+
 
 def philox_uniform(seed: int, counter: int) -> float:
     """Philox-4x32-10 keyed by `seed`, counter `counter`; first word -> [0, 1)."""
@@ -989,6 +992,84 @@ class ReferenceOps:
             pick = int((cum <= u * float(cum[-1])).sum())
             out[i] = int(indices[min(pick, len(indices) - 1)])
         return out.to(logits.device)
+
+    # ---------------------------------------------------------------- several answers to one prompt
+
+    def row_set(self, tensors, token_axes=None, targets=None):
+        return RowSet(tensors, token_axes, targets)
+
+    def copy_rows(self, rows, sources, targets, tokens=None):
+        """Row by row; see `HipOps.copy_rows`."""
+        for s, d, n in rows.pairs(sources, targets, tokens).tolist():
+            for t, to, axis in zip(rows.tensors, rows.targets, rows.token_axes):
+                if axis is None or n < 0:
+                    to[d].copy_(t[s])
+                else:
+                    to[d].narrow(axis - 1, 0, n).copy_(t[s].narrow(axis - 1, 0, n))
+
+    def token_history(self, slots, capacity):
+        return TokenHistory(torch.zeros(slots, capacity, 2, dtype=torch.int32, device=self.device),
+                            torch.zeros(slots, dtype=torch.int32, device=self.device))
+
+    def start_history(self, history, slots, prompts, outputs=None, last=None):
+        for i, slot in enumerate(slots):
+            entries = TokenHistory.distinct(prompts[i], () if outputs is None else outputs[i])
+            history.entries[slot, :len(entries)] = torch.from_numpy(entries).to(history.entries.device)
+            history.used[slot] = len(entries)
+            if last is not None:
+                last[slot] = -1
+
+    def logit_rules(self, vocab, rows=None, slots=None, repetition=None, presence=None, frequency=None, biases=None, mask_rows=None):
+        if rows is None:
+            rows = next(len(v) for v in (slots, repetition, presence, frequency, biases, mask_rows) if v is not None)
+        rules = LogitRules(vocab, rows, slots, repetition, presence, frequency, biases, mask_rows)
+        rules.device_words = torch.from_numpy(rules.flat)
+        return rules
+
+    def adjust_logits(self, logits, rules, history=None, last=None, masks=None):
+        """Row by row, in float32; see `HipOps.adjust_logits`."""
+        head, tokens, values = rules.pieces(rules.flat)
+        head = head.reshape(rules.rows, rules.WORDS)
+        numbers = head[:, 1:4].view("float32")
+        for i in range(rules.rows):
+            row, slot = logits[i], int(head[i, 0])
+            if slot >= 0:
+                n, token = int(history.used[slot]), int(last[slot])
+                if token >= 0:
+                    at = (history.entries[slot, :n, 0] == token).nonzero().flatten()
+                    if at.numel():
+                        history.entries[slot, at[0], 1] += 2
+                    else:
+                        history.entries[slot, n] = torch.tensor([token, 2], dtype=torch.int32)
+                        history.used[slot] = n = n + 1
+                ids, info = history.entries[slot, :n, 0].long(), history.entries[slot, :n, 1]
+                rho, presence, frequency = (float(v) for v in numbers[i])
+                times = (info >> 1).float()
+                x = row[ids]
+                y = torch.where(x > 0, x / rho, x * rho)
+                row[ids] = y - (frequency * times + torch.where(times > 0, presence, 0.0))
+            a, b = int(head[i, 4]), int(head[i, 5])
+            if b > a:
+                ids = torch.from_numpy(tokens[a:b].astype("int64")).to(logits.device)
+                add = torch.from_numpy(values[a:b].view("float32").copy()).to(logits.device)
+                row[ids] = torch.where(torch.isneginf(add), add, row[ids] + add)
+            if head[i, 6] >= 0:
+                bits = (masks[int(head[i, 6])].unsqueeze(-1) >> torch.arange(32, dtype=torch.int32, device=masks.device)) & 1
+                row[bits.reshape(-1)[:rules.vocab] == 0] = float("-inf")
+        return logits
+
+    def log_probs(self, logits, tokens, top=0):
+        """See `HipOps.log_probs`."""
+        x = torch.where(torch.isnan(logits), float("-inf"), logits)
+        m = x.max(dim=1, keepdim=True).values
+        d = torch.where(x == m, torch.where(torch.isneginf(m), float("-inf"), 0.0), x - torch.where(torch.isneginf(m), 0.0, m))
+        lp = d - torch.log(torch.exp(d).sum(1, keepdim=True).clamp(min=1.0))
+        ok = (tokens >= 0) & (tokens < logits.shape[1])
+        out = torch.where(ok, lp.gather(1, torch.where(ok, tokens, 0).long()[:, None])[:, 0], float("-inf"))
+        if not top:
+            return out, None, None
+        ids = torch.sort(x, dim=1, descending=True, stable=True).indices[:, :top]
+        return out, ids.to(torch.int32), lp.gather(1, ids)
 
     def synchronize(self):
         if self.device.type == "cuda":
