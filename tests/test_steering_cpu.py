@@ -41,7 +41,8 @@ def test_how_rows_lie_is_what_the_kernel_is_told():
     rows = RowSet([k, torch.zeros(5, 3, dtype=torch.bfloat16), torch.zeros(5, 7, dtype=torch.uint8)], [2, None, None])
     assert rows.words[0, 2:].tolist() == [272 * 4, 272 * 4, 16 * 8 * 4, 8 * 4, 2, 16]
     assert rows.words[1, 2:].tolist() == [6, 6, 6, 0, 1, 2] and rows.words[2, 7] == 1
-    assert rows.row_bytes == 1024 + 6 + 7 and rows.largest == 1024 and rows.places == 16
+    assert rows.row_bytes == 1024 + 6 + 7 and rows.places == 16
+    assert rows.units(-1) == 64 and rows.units(3) == 12 and rows.units(0) == 7
 
 
 @pytest.mark.parametrize("what, sources, targets, tokens", [

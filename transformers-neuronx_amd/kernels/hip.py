@@ -233,7 +233,7 @@ _SIGNATURES = {
         "tnx_decode_layers": [_c_void_p, _c_int, _c_void_p],
     },
     "rows": {
-        "tnx_copy_rows": [_c_void_p, _c_int, _c_void_p, _c_int, _c_ll, _c_void_p],
+        "tnx_copy_rows": [_c_void_p, _c_int, _c_void_p, _c_int, _c_void_p, _c_ll, _c_void_p],
     },
     "steering": {
         "tnx_start_history": [_c_void_p, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_void_p],
@@ -2915,14 +2915,17 @@ class HipOps:
         the tensor counts tokens, or whole (`tokens` None, or a tensor without a token axis). What lies behind them stays as it
         was. The rows are lists on the host; a source may be named several times, a target once and not as a source too."""
         pairs = rows.pairs(sources, targets, tokens)
-        if len(pairs) == 0:
-            return
         if rows.table is None:
             raise ValueError("this set of rows was not made by row_set")
+        units = rows.units(max(n for _, n, _ in pairs) if pairs and tokens is not None else -1)
+        if not pairs or units == 0:
+            return
         self._on_this_device(rows.device, "rows")
-        dev = self._from_host(pairs.reshape(-1), "copy_rows")
-        self._call("rows", "tnx_copy_rows", _ptr(rows.table), len(rows.tensors), _ptr(dev), len(pairs), rows.largest, _stream(),
-                   work=lambda: (f"{len(pairs)} rows", 2 * len(pairs) * rows.row_bytes, 0))
+        groups, into = rows.groups(pairs)
+        dev = self._from_host(np.array([w for g in groups for w in g] + into, dtype=np.int32), "copy_rows")
+        self._call("rows", "tnx_copy_rows", _ptr(rows.table), len(rows.tensors), _ptr(dev), len(groups),
+                   dev.data_ptr() + 16 * len(groups), units, _stream(),
+                   work=lambda: (f"{len(groups)} to {len(pairs)} rows", (len(groups) + len(pairs)) * rows.row_bytes, 0))
 
     def token_history(self, slots: int, capacity: int) -> TokenHistory:
         """Empty histories for `slots` sequences of at most `capacity` distinct tokens."""

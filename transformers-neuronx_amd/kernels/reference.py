@@ -1000,7 +1000,7 @@ class ReferenceOps:
 
     def copy_rows(self, rows, sources, targets, tokens=None):
         """Row by row; see `HipOps.copy_rows`."""
-        for s, d, n in rows.pairs(sources, targets, tokens).tolist():
+        for s, n, d in rows.pairs(sources, targets, tokens):
             for t, to, axis in zip(rows.tensors, rows.targets, rows.token_axes):
                 if axis is None or n < 0:
                     to[d].copy_(t[s])

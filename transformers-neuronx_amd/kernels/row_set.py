@@ -1,5 +1,5 @@
 """Rows of several tensors that are copied together: what a page (or a slot) is across all layers of a cache."""
-from typing import List, Optional, Sequence
+from typing import List, Optional, Sequence, Tuple
 
 import numpy as np
 import torch
@@ -50,9 +50,8 @@ class RowSet:
                 run = shape[axis] * inner
                 outer = row // run
                 places.add(shape[axis])
-            distances = [t.data_ptr(), to.data_ptr(), run]
-            distances += [x.stride(0) * item for x in (t, to) if x.shape[0] > 1]
-            grain = next(g for g in (16, 4, 2, 1) if all(d % g == 0 for d in distances))
+            distances = [t.data_ptr(), to.data_ptr(), run] + [x.stride(0) * item for x in (t, to) if x.shape[0] > 1]
+            grain = next(g for g in (16, 4, 2, 1) if all(d % g == 0 for d in distances + ([] if g == 16 else [inner])))
             words.append([t.data_ptr(), to.data_ptr(), t.stride(0) * item, to.stride(0) * item, run, inner, outer, grain])
         if len(places) > 1:
             raise ValueError(f"the token axes of a set of rows are of one length, got {sorted(places)}")
@@ -60,40 +59,55 @@ class RowSet:
         self.num_rows = min(t.shape[0] for t in self.tensors)
         self.num_target_rows = min(t.shape[0] for t in self.targets)
         self.row_bytes = sum(w[4] * w[6] for w in words)
-        self.largest = max(w[4] * w[6] for w in words)
+        self._shapes = sorted({tuple(w[4:]) for w in words})
         self.words = np.array(words, dtype=np.int64)
         self.table: Optional[torch.Tensor] = None          # the words on the device, put there by the backend
 
-    def pairs(self, sources: Sequence[int], targets: Sequence[int], tokens=None) -> np.ndarray:
-        """int32 `[n, 3]` (source, target, tokens; -1: all), checked: rows there are, no target named twice, and within the
-        same tensors no target that is a source."""
-        src, dst = np.asarray(sources, dtype=np.int64).reshape(-1), np.asarray(targets, dtype=np.int64).reshape(-1)
-        n = src.size
-        if dst.size != n:
-            raise ValueError(f"{n} sources and {dst.size} targets")
-        out = np.empty((n, 3), dtype=np.int32)
+    def units(self, tokens: int) -> int:
+        """Pieces of at most 16 bytes in what is copied of the largest row where it holds `tokens` tokens (below zero: all)."""
+        most = 0
+        for run, inner, outer, grain in self._shapes:
+            length = run if tokens < 0 or inner == 0 else min(run, tokens * inner)
+            most = max(most, -(-length * outer // grain) if length == run else -(-length // grain) * outer)
+        return most
+
+    def pairs(self, sources: Sequence[int], targets: Sequence[int], tokens=None) -> List[Tuple[int, int, int]]:
+        """(source, tokens, target), tokens -1 for all, ordered by them, and checked: rows there are, no target named twice, and
+        within the same tensors no target that is a source."""
+        src, dst = [int(s) for s in sources], [int(d) for d in targets]
+        n = len(src)
+        if len(dst) != n:
+            raise ValueError(f"{n} sources and {len(dst)} targets")
         if n == 0:
-            return out
+            return []
         for what, rows, most in (("source", src, self.num_rows), ("target", dst, self.num_target_rows)):
-            if rows.min() < 0 or rows.max() >= most:
-                bad = rows.min() if rows.min() < 0 else rows.max()
-                raise ValueError(f"{what} row {int(bad)} is outside the {most} rows there are")
-        if n > 1 and np.unique(dst).size != n:
+            low, high = min(rows), max(rows)
+            if low < 0 or high >= most:
+                raise ValueError(f"{what} row {low if low < 0 else high} is outside the {most} rows there are")
+        into = set(dst)
+        if len(into) != n:
             raise ValueError("a target row is named twice")
-        if self.in_place and np.isin(dst, src).any():
+        if self.in_place and not into.isdisjoint(src):
             raise ValueError("a row is both source and target")
-        out[:, 0], out[:, 1] = src, dst
         if tokens is None:
-            out[:, 2] = -1
-            return out
-        if self.places is None:
-            raise ValueError("no tensor of this set counts tokens")
-        held = np.asarray(tokens, dtype=np.int64).reshape(-1)
-        if held.size == 1:
-            held = np.broadcast_to(held, (n,))
-        if held.size != n:
-            raise ValueError(f"{n} pairs of rows and {held.size} numbers of tokens")
-        if held.min() < 0 or held.max() > self.places:
-            raise ValueError(f"a row holds 0 to {self.places} tokens, got {int(held.min())} to {int(held.max())}")
-        out[:, 2] = held
-        return out
+            held = [-1] * n
+        else:
+            if self.places is None:
+                raise ValueError("no tensor of this set counts tokens")
+            held = [int(tokens)] * n if isinstance(tokens, (int, np.integer)) else [int(t) for t in tokens]
+            if len(held) != n:
+                raise ValueError(f"{n} pairs of rows and {len(held)} numbers of tokens")
+            if min(held) < 0 or max(held) > self.places:
+                raise ValueError(f"a row holds 0 to {self.places} tokens, got {min(held)} to {max(held)}")
+        return sorted(zip(src, held, dst))
+
+    @staticmethod
+    def groups(pairs: List[Tuple[int, int, int]]) -> Tuple[List[List[int]], List[int]]:
+        """([source, tokens, first target, targets] of every source with its tokens, the targets)."""
+        heads: List[List[int]] = []
+        for i, (s, n, _) in enumerate(pairs):
+            if heads and heads[-1][0] == s and heads[-1][1] == n:
+                heads[-1][3] += 1
+            else:
+                heads.append([s, n, i, 1])
+        return heads, [d for _, _, d in pairs]
