@@ -25,14 +25,26 @@ struct RowTensor {
 #define ROW_THREADS 256
 #define ROW_UNITS 4           // units of a thread that are asked for together, before any is stored
 
-// The first `bytes` (below 16) of a unit, by pieces of the sizes that make them up.
+#define ROW_LINE 128          // bytes that memory is read by; a half of it is what it is written by at least
+
+// The first `bytes` (0 to 15) of `v`, and the rest of `w`.
+__device__ __forceinline__ tnx_u32x4 joined(tnx_u32x4 v, tnx_u32x4 w, unsigned bytes) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int here = min(max((int)bytes - 4 * j, 0), 4);
+    const unsigned mask = here == 4 ? ~0u : (1u << (8 * here)) - 1u;
+    w[j] = (v[j] & mask) | (w[j] & ~mask);
+  }
+  return w;
+}
+
+// The first `bytes` (0 to 15) of a unit stored, by pieces of the sizes that make them up.
 __device__ __forceinline__ void store_part(char* d, tnx_u32x4 v, unsigned bytes) {
-  unsigned long long w[2] = {((unsigned long long)v[1] << 32) | v[0], ((unsigned long long)v[3] << 32) | v[2]};
-  unsigned long long x = w[0];
+  unsigned long long x = ((unsigned long long)v[1] << 32) | v[0];
   if (bytes & 8) {
     *(unsigned long long*)d = x;
     d += 8;
-    x = w[1];
+    x = ((unsigned long long)v[3] << 32) | v[2];
   }
   if (bytes & 4) {
     *(unsigned*)d = (unsigned)x;
@@ -46,35 +58,53 @@ __device__ __forceinline__ void store_part(char* d, tnx_u32x4 v, unsigned bytes)
   }
   if (bytes & 1) *d = (char)x;
 }
-template <typename V>
-__device__ __forceinline__ void store_part(char*, V, unsigned) {}
 
-// `length` bytes of each of `runs` runs that lie `stride` bytes apart, to every target. A unit is a V; the last of a run may be a
-// part of one where V is 16 bytes (runs there are whole units long, so all of it can be read), and never is for smaller V, of which
-// a place holds a whole number.
-template <typename V>
+// `length` bytes of each of `runs` runs that lie `stride` bytes apart, to every target, by units of a V. A run may end inside a unit
+// where V is 16 bytes (it can be read whole: runs are whole units long); of a smaller V a place holds a whole number.
+//
+// FILL: what a run's last line lacks is filled up with what the target has there. Values turned inside a page are runs of 128 bytes,
+// of which a page that is not full moves a part; memory then reads, changes and writes back what it is given a part of. Values of 32
+// layers of 32 heads of 128, page 64, 8 pages to 24, in us: whole pages 115; 45 tokens (90 bytes of 128) parts 233, filled up 200;
+// 32 tokens (64 bytes) parts 87, filled up 195; 16 tokens 110 and 196. So lines are filled up where more than half of one is moved.
+template <typename V, bool FILL>
 __device__ __forceinline__ void copy_runs(const char* from, char* to, long long to_stride, const int* targets, int num_targets,
                                           long long stride, unsigned length, unsigned runs) {
   constexpr unsigned SIZE = sizeof(V);
-  const unsigned per_run = (length + SIZE - 1) / SIZE, units = per_run * runs;
+  const unsigned wide = FILL ? (unsigned)min((long long)(length + ROW_LINE - 1) / ROW_LINE * ROW_LINE, stride) : length;
+  const unsigned per_run = (wide + SIZE - 1) / SIZE, units = per_run * runs;
   for (unsigned u0 = blockIdx.x * (ROW_THREADS * ROW_UNITS) + threadIdx.x; u0 < units; u0 += gridDim.x * (ROW_THREADS * ROW_UNITS)) {
     V v[ROW_UNITS];
     long long at[ROW_UNITS];
-    unsigned left[ROW_UNITS];
+    unsigned mine[ROW_UNITS];        // bytes of the unit that are the source's
 #pragma unroll
     for (int k = 0; k < ROW_UNITS; ++k) {
       const unsigned u = min(u0 + k * ROW_THREADS, units - 1);
       const unsigned o = u / per_run, in = (u - o * per_run) * SIZE;
       at[k] = o * stride + in;
-      left[k] = u0 + k * ROW_THREADS < units ? min(length - in, SIZE) : 0;
+      mine[k] = in < length ? min(length - in, SIZE) : 0;
       v[k] = *(const V*)(from + at[k]);
     }
     for (int i = 0; i < num_targets; ++i) {
       char* d = to + targets[i] * to_stride;
+      if constexpr (FILL) {
+        V w[ROW_UNITS];
 #pragma unroll
-      for (int k = 0; k < ROW_UNITS; ++k) {
-        if (left[k] == SIZE) *(V*)(d + at[k]) = v[k];
-        else if (left[k]) store_part(d + at[k], v[k], left[k]);
+        for (int k = 0; k < ROW_UNITS; ++k) {
+          w[k] = v[k];
+          if (mine[k] < SIZE) w[k] = *(const V*)(d + at[k]);
+        }
+#pragma unroll
+        for (int k = 0; k < ROW_UNITS; ++k) {
+          if (mine[k] < SIZE) w[k] = joined(v[k], w[k], mine[k]);
+          if (u0 + k * ROW_THREADS < units) *(V*)(d + at[k]) = w[k];
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < ROW_UNITS; ++k) {
+          if (u0 + k * ROW_THREADS >= units) continue;
+          if (mine[k] == SIZE) *(V*)(d + at[k]) = v[k];
+          else if constexpr (SIZE == 16) store_part(d + at[k], v[k], mine[k]);
+        }
       }
     }
   }
@@ -95,10 +125,12 @@ copy_rows_kernel(const RowTensor* __restrict__ tensors, const int4* __restrict__
     runs = 1;
   }
   const int* to = targets + g.z;
-  if (t.grain == 16) copy_runs<tnx_u32x4>(from, t.to, t.to_stride, to, g.w, t.run, length, runs);
-  else if (t.grain == 4) copy_runs<unsigned>(from, t.to, t.to_stride, to, g.w, t.run, length, runs);
-  else if (t.grain == 2) copy_runs<unsigned short>(from, t.to, t.to_stride, to, g.w, t.run, length, runs);
-  else copy_runs<unsigned char>(from, t.to, t.to_stride, to, g.w, t.run, length, runs);
+  const bool fill = runs > 1 && length % ROW_LINE > ROW_LINE / 2;
+  if (t.grain == 16 && fill) copy_runs<tnx_u32x4, true>(from, t.to, t.to_stride, to, g.w, t.run, length, runs);
+  else if (t.grain == 16) copy_runs<tnx_u32x4, false>(from, t.to, t.to_stride, to, g.w, t.run, length, runs);
+  else if (t.grain == 4) copy_runs<unsigned, false>(from, t.to, t.to_stride, to, g.w, t.run, length, runs);
+  else if (t.grain == 2) copy_runs<unsigned short, false>(from, t.to, t.to_stride, to, g.w, t.run, length, runs);
+  else copy_runs<unsigned char, false>(from, t.to, t.to_stride, to, g.w, t.run, length, runs);
 }
 
 // `units`: of 16 bytes or less, in what is copied of the set's largest row (below 2^31).
