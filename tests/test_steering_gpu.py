@@ -227,17 +227,23 @@ def test_log_probs(ops, rows, vocab, top):
 
 
 @pytest.mark.parametrize("vocab", [5, 300, 5000, 50272])
-@pytest.mark.parametrize("how", ["equal", "few values", "rising", "falling", "barred", "blocks"])
+@pytest.mark.parametrize("how", ["equal", "few values", "rising", "falling", "barred", "blocks", "crowd"])
 def test_log_probs_of_ties_and_orders(ops, how, vocab):
     """Rows whose largest logits are many, alike, or all in one place."""
     i = torch.arange(vocab, device="cuda", dtype=torch.float32)
     row = {"equal": torch.zeros_like(i), "few values": (i * 7) % 3, "rising": i / vocab * 9, "falling": -i / vocab * 9,
            "barred": torch.where(i % 97 == 3, i / vocab, torch.tensor(float("-inf"), device="cuda")),
-           "blocks": torch.where((i % 1024) < 4, 5 + i / vocab, -i / vocab)}[how]
+           "blocks": torch.where((i % 1024) < 4, 5 + i / vocab, -i / vocab),
+           "crowd": torch.where(i // 16 % 256 < 8, 5 + i * 7919 % 1000 / 1000, -i / vocab)}[how]
     logits = torch.stack([row, row.roll(1), -row])
     tokens = torch.tensor([0, vocab // 2, vocab - 1], dtype=torch.int32, device="cuda")
     top = min(20, vocab)
-    _check_log_probs(logits, tokens, top, ops.log_probs(logits, tokens, top))
+    few = ops.log_probs(logits, tokens, top)
+    _check_log_probs(logits, tokens, top, few)
+    # many rows are worked on by smaller blocks
+    many = ops.log_probs(logits.repeat(200, 1), tokens.repeat(200), top)
+    for k in (0, 199):
+        _check_log_probs(logits, tokens, top, [t[3 * k:3 * k + 3] for t in many])
 
 
 @pytest.mark.parametrize("vocab", [3, 40, 3000])

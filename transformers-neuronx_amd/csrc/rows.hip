@@ -64,8 +64,12 @@ __device__ __forceinline__ void store_part(char* d, tnx_u32x4 v, unsigned bytes)
 //
 // FILL: what a run's last line lacks is filled up with what the target has there. Values turned inside a page are runs of 128 bytes,
 // of which a page that is not full moves a part; memory then reads, changes and writes back what it is given a part of. Values of 32
-// layers of 32 heads of 128, page 64, 8 pages to 24, in us: whole pages 115; 45 tokens (90 bytes of 128) parts 233, filled up 200;
-// 32 tokens (64 bytes) parts 87, filled up 195; 16 tokens 110 and 196. So lines are filled up where more than half of one is moved.
+// layers of 32 heads of 128, page 64, 8 pages to 24, in us: whole pages 91; 40 tokens (80 bytes of 128) parts 233, filled up 168;
+// 32 tokens (64 bytes) parts 70, filled up 195; 16 tokens 110 and 196. So lines are filled up where more than half of one is moved.
+//
+// What bounds it is memory: stores are marked as not read again soon, which leaves the caches to the sources. 20 whole pages of
+// OPT-6.7b to 20 others, 0.67 GB read and as much written: 5.6 TB/s, 4.7 with plain stores, 5.3 with loads marked so too (as is right
+// for what fills up lines, 199 -> 168 us); one to eight units a thread asked for together are alike within 3%.
 template <typename V, bool FILL>
 __device__ __forceinline__ void copy_runs(const char* from, char* to, long long to_stride, const int* targets, int num_targets,
                                           long long stride, unsigned length, unsigned runs) {
@@ -91,18 +95,18 @@ __device__ __forceinline__ void copy_runs(const char* from, char* to, long long 
 #pragma unroll
         for (int k = 0; k < ROW_UNITS; ++k) {
           w[k] = v[k];
-          if (mine[k] < SIZE) w[k] = *(const V*)(d + at[k]);
+          if (mine[k] < SIZE) w[k] = __builtin_nontemporal_load((const V*)(d + at[k]));
         }
 #pragma unroll
         for (int k = 0; k < ROW_UNITS; ++k) {
           if (mine[k] < SIZE) w[k] = joined(v[k], w[k], mine[k]);
-          if (u0 + k * ROW_THREADS < units) *(V*)(d + at[k]) = w[k];
+          if (u0 + k * ROW_THREADS < units) __builtin_nontemporal_store(w[k], (V*)(d + at[k]));
         }
       } else {
 #pragma unroll
         for (int k = 0; k < ROW_UNITS; ++k) {
           if (u0 + k * ROW_THREADS >= units) continue;
-          if (mine[k] == SIZE) *(V*)(d + at[k]) = v[k];
+          if (mine[k] == SIZE) __builtin_nontemporal_store(v[k], (V*)(d + at[k]));
           else if constexpr (SIZE == 16) store_part(d + at[k], v[k], mine[k]);
         }
       }

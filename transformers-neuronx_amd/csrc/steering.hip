@@ -125,62 +125,218 @@ __device__ __forceinline__ unsigned long long order_key(float x, int idx) {
   return ((unsigned long long)u << 32) | (unsigned)(~(unsigned)idx);
 }
 
-#define SCORE_THREADS 256
+// exp(d) for d <= 0 by the hardware's power of two; log2(e) in two parts, so that only the roundings of d and of the power's argument
+// are left: 2^-24 of |d| each, and what is far below the largest adds little.
+__device__ __forceinline__ float exp_of(float d) {
+  const float hi = 1.44269502162933349609375f, lo = 1.92596299112661746887e-8f;
+  return __builtin_amdgcn_exp2f(fmaf(d, hi, d * lo));
+}
 
-__global__ void __launch_bounds__(SCORE_THREADS)
+// A row read four logits at a time from the boundary of 16 bytes at or before it: quad q holds elements 4 q - lead to 4 q - lead + 3;
+// what lies outside the row reads as -inf. A NaN reads as -inf as well.
+struct Quads {
+  const float* row;
+  int vocab, lead, count;
+  __device__ __forceinline__ Quads(const float* r, int v)
+      : row(r), vocab(v), lead((int)(((uintptr_t)r >> 2) & 3)), count((v + (int)(((uintptr_t)r >> 2) & 3) + 3) / 4) {}
+  __device__ __forceinline__ int first(int q) const { return 4 * q - lead; }
+  __device__ __forceinline__ f32x4 operator()(int q) const {
+    const int i = 4 * q - lead;
+    f32x4 x;
+    if (q < count && i >= 0 && i + 3 < vocab) {
+      x = *(const f32x4*)(row + i);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = q < count && i + e >= 0 && i + e < vocab ? row[i + e] : -INFINITY;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = fmaxf(x[e], -INFINITY);
+    return x;
+  }
+};
+
+#define SCORE_GROUPS 256       // groups of threads whose largest logits are ranked against one another
+#define SCORE_GATHER 1024      // the most logits that are gathered for the alternatives
+#define SCORE_MOST_TOP 32
+#define SCORE_WIDE_ROWS 512
+
+// One block of THREADS a row, one pass over it with a running maximum and sum.
+//
+// The alternatives come from the same pass: a thread notes its largest logit, and as many groups of threads as alternatives are
+// wanted, those with the largest logits, hold all of them (of the others each group's best is already beaten by so many). Only
+// the logits of these groups are looked at again, and those of them that are no smaller than the last group's best, hardly more than
+// the alternatives themselves, are ranked in LDS. Should they be more than fit (the best of a long row all in a few threads' places),
+// the alternatives are found one by one, each with a pass of its own.
+template <int THREADS, bool TOP>
+__global__ void __launch_bounds__(THREADS)
 log_probs_kernel(const float* __restrict__ logits, const int* __restrict__ tokens, float* __restrict__ out, int* __restrict__ top_tokens,
                  float* __restrict__ top_out, int top, int vocab) {
-  __shared__ float scratch[SCORE_THREADS / 64];
-  __shared__ unsigned long long best[SCORE_THREADS / 64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const float* row = logits + (size_t)blockIdx.x * vocab;
-  float m = -INFINITY;
-  for (int i = threadIdx.x; i < vocab; i += SCORE_THREADS) m = fmaxf(m, row[i]);
+  constexpr int WAVES = THREADS / 64, PER_GROUP = THREADS / SCORE_GROUPS;
+  __shared__ float scratch[WAVES], sums[WAVES];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const Quads quads(logits + (size_t)blockIdx.x * vocab, vocab);
+  const float* row = quads.row;
+
+  float m = -INFINITY, s = 0.f;
+  int at = tid;                       // the quads among which the thread's largest logit came first
+  for (int q0 = tid; q0 < quads.count; q0 += 4 * THREADS) {
+    f32x4 v[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = quads(q0 + k * THREADS);
+    float here = v[0][0];
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) here = fmaxf(here, v[k][e]);
+    if (here > m) {
+      s *= m > -INFINITY ? exp_of(m - here) : 0.f;
+      m = here;
+      at = q0;
+    }
+    const float base = fmaxf(m, -3.402823466e38f);       // -inf less -inf would be no number
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s += exp_of(v[k][e] - base);
+  }
+  const float mine = m;
   m = wave_max(m);
   if (lane == 0) scratch[wave] = m;
   __syncthreads();
-  for (int w = 0; w < SCORE_THREADS / 64; ++w) m = fmaxf(m, scratch[w]);
-  float s = 0.f;
-  for (int i = threadIdx.x; i < vocab; i += SCORE_THREADS) {
-    const float x = row[i];
-    s += x == m ? 1.f : x > -INFINITY ? expf(x - m) : 0.f;
+  m = scratch[0];
+#pragma unroll
+  for (int w = 1; w < WAVES; ++w) m = fmaxf(m, scratch[w]);
+  if (m < INFINITY) {
+    s = mine > -INFINITY ? s * exp_of(mine - m) : 0.f;
+  } else {                            // those at +inf are counted
+    s = 0.f;
+    for (int q = tid; q < quads.count; q += THREADS) {
+      const f32x4 x = quads(q);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s += x[e] == INFINITY ? 1.f : 0.f;
+    }
   }
-  const float log_l = logf(block_sum<SCORE_THREADS / 64>(s, scratch));
-  if (threadIdx.x == 0) {
+  const float log_l = logf(block_sum<WAVES>(s, sums));
+  if (tid == 0) {
     const int t = tokens[blockIdx.x];
     out[blockIdx.x] = t >= 0 && t < vocab ? log_prob_of(row[t], m, log_l) : -INFINITY;
   }
-  unsigned long long below = ~0ull;
-  for (int k = 0; k < top; ++k) {
-    unsigned long long b = 0;
-    for (int i = threadIdx.x; i < vocab; i += SCORE_THREADS) {
-      const unsigned long long key = order_key(row[i], i);
-      if (key < below && key > b) b = key;
+  if constexpr (TOP) {
+    __shared__ unsigned long long best[SCORE_GROUPS], gathered[SCORE_GATHER], one[WAVES];
+    __shared__ int winners[SCORE_MOST_TOP], num_winners, num_gathered;
+    __shared__ unsigned long long least;
+    // the thread's best as a key (its logit, then the lower token id), and its group's
+    unsigned long long key = 0;
+    if (tid < quads.count) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const f32x4 x = quads(at + k * THREADS);
+        const int i = quads.first(at + k * THREADS);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (i + e >= 0 && i + e < vocab) {
+            const unsigned long long other = order_key(x[e], i + e);
+            key = other > key ? other : key;
+          }
+      }
     }
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-      const unsigned long long other = __shfl_xor(b, o, 64);
-      b = other > b ? other : b;
+    for (int o = 1; o < PER_GROUP; o <<= 1) {
+      const unsigned long long other = __shfl_xor(key, o, 64);
+      key = other > key ? other : key;
+    }
+    if (tid % PER_GROUP == 0) best[tid / PER_GROUP] = key;
+    if (tid == 0) {
+      num_winners = num_gathered = 0;
+      least = 0;
     }
     __syncthreads();
-    if (lane == 0) best[wave] = b;
+    if (tid < SCORE_GROUPS && best[tid] != 0) {          // (0: a group without logits)
+      const unsigned long long b = best[tid];
+      int rank = 0;
+      for (int j = 0; j < SCORE_GROUPS; ++j) rank += best[j] > b ? 1 : 0;
+      if (rank < top) {
+        winners[rank] = tid;
+        atomicAdd(&num_winners, 1);
+      }
+      if (rank == top - 1) least = b;                    // (fewer groups than alternatives: everything is gathered)
+    }
     __syncthreads();
-    for (int w = 0; w < SCORE_THREADS / 64; ++w) b = best[w] > b ? best[w] : b;
-    below = b;
-    if (threadIdx.x == 0) {
-      const int t = (int)(~(unsigned)b);
-      top_tokens[(size_t)blockIdx.x * top + k] = t;
-      top_out[(size_t)blockIdx.x * top + k] = log_prob_of(row[t], m, log_l);
+    // group g's quads are those of its threads: k * THREADS + PER_GROUP * g + j
+    const int rounds = (quads.count + THREADS - 1) / THREADS * PER_GROUP;
+    const unsigned long long floor_key = least;
+    for (int w = wave; w < num_winners; w += WAVES)
+      for (int n = lane; n < rounds; n += 64) {
+        const int q = n / PER_GROUP * THREADS + PER_GROUP * winners[w] + n % PER_GROUP;
+        const f32x4 x = quads(q);
+        const int i = quads.first(q);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (q < quads.count && i + e >= 0 && i + e < vocab) {
+            const unsigned long long k = order_key(x[e], i + e);
+            if (k >= floor_key) {
+              const int to = atomicAdd(&num_gathered, 1);
+              if (to < SCORE_GATHER) gathered[to] = k;
+            }
+          }
+      }
+    __syncthreads();
+    const int n = num_gathered;
+    int* ids = top_tokens + (size_t)blockIdx.x * top;
+    float* values = top_out + (size_t)blockIdx.x * top;
+    if (n <= SCORE_GATHER) {
+      for (int c = tid; c < n; c += THREADS) {
+        const unsigned long long k = gathered[c];
+        int rank = 0;
+        for (int j = 0; j < n; ++j) rank += gathered[j] > k ? 1 : 0;
+        if (rank < top) {
+          const int t = (int)(~(unsigned)k);
+          ids[rank] = t;
+          values[rank] = log_prob_of(row[t], m, log_l);
+        }
+      }
+    } else {
+      unsigned long long below = ~0ull;
+      for (int r = 0; r < top; ++r) {
+        unsigned long long b = 0;
+        for (int i = tid; i < vocab; i += THREADS) {
+          const unsigned long long k = order_key(row[i], i);
+          if (k < below && k > b) b = k;
+        }
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) {
+          const unsigned long long other = __shfl_xor(b, o, 64);
+          b = other > b ? other : b;
+        }
+        __syncthreads();
+        if (lane == 0) one[wave] = b;
+        __syncthreads();
+        for (int w = 0; w < WAVES; ++w) b = one[w] > b ? one[w] : b;
+        below = b;
+        if (tid == 0) {
+          const int t = (int)(~(unsigned)b);
+          ids[r] = t;
+          values[r] = log_prob_of(row[t], m, log_l);
+        }
+      }
     }
   }
 }
 
+template <int THREADS>
+static void launch_log_probs(const float* logits, const int* tokens, float* out, int* top_tokens, float* top_out, int top, int rows, int vocab,
+                             hipStream_t stream) {
+  if (top) log_probs_kernel<THREADS, true><<<rows, THREADS, 0, stream>>>(logits, tokens, out, top_tokens, top_out, top, vocab);
+  else log_probs_kernel<THREADS, false><<<rows, THREADS, 0, stream>>>(logits, tokens, out, top_tokens, top_out, top, vocab);
+}
+
 extern "C" int tnx_log_probs(const float* logits, const int* tokens, float* out, int* top_tokens, float* top_out, int top, int rows,
                              int vocab, hipStream_t stream) {
-  TNX_REQUIRE(rows >= 0 && vocab > 0 && top >= 0 && top <= 32 && top <= vocab, "log_probs: bad sizes rows=%d vocab=%d top=%d", rows, vocab,
-              top);
+  TNX_REQUIRE(rows >= 0 && vocab > 0 && vocab < (1 << 30) && top >= 0 && top <= SCORE_MOST_TOP && top <= vocab,
+              "log_probs: bad sizes rows=%d vocab=%d top=%d", rows, vocab, top);
   if (rows == 0) return 0;
-  log_probs_kernel<<<rows, SCORE_THREADS, 0, stream>>>(logits, tokens, out, top_tokens, top_out, top, vocab);
+  if (rows <= SCORE_WIDE_ROWS) launch_log_probs<1024>(logits, tokens, out, top_tokens, top_out, top, rows, vocab, stream);
+  else launch_log_probs<256>(logits, tokens, out, top_tokens, top_out, top, rows, vocab, stream);
   TNX_CHECK_LAUNCH("log_probs");
   return 0;
 }
