@@ -54,55 +54,117 @@ __device__ __forceinline__ float penalised(float x, const RowRules& r, int info)
   return x - (r.frequency * (float)times + (times > 0 ? r.presence : 0.f));
 }
 
-// One block a row. Every logit is written by one thread at a time: history entries name distinct tokens, so do a row's
-// biases, a barrier lies between the two, and tokens that the mask bars are left to the last loop, which writes nothing else.
-__global__ void __launch_bounds__(256)
+#define ADJUST_THREADS 1024
+#define ADJUST_AHEAD 4         // history entries (or quads of barred tokens) of a thread that are on their way together
+
+// Block 0 of a row does what names single tokens, its history and its biases; the others write -inf where the mask bars a token,
+// ADJUST_THREADS * ADJUST_AHEAD quads of logits each. A logit is written by one thread at a time: history entries name distinct tokens,
+// so do a row's biases, a barrier lies between the two, and barred tokens are left to the other blocks, which write nothing else.
+//
+// Of a row's logits only those named are read, and only those barred written: what bounds a batch without masks is the way from the
+// rules to the history's entries, to the logits and back, three trips to memory one behind the other, not their bytes.
+__global__ void __launch_bounds__(ADJUST_THREADS)
 adjust_logits_kernel(float* __restrict__ logits, const RowRules* __restrict__ rules, const int* __restrict__ bias_tokens,
                      const float* __restrict__ bias_values, int2* __restrict__ entries, int* __restrict__ used, int capacity,
                      const int* __restrict__ last, const unsigned* __restrict__ masks, int words, int vocab) {
-  const RowRules r = rules[blockIdx.x];
-  float* row = logits + (size_t)blockIdx.x * vocab;
+  const RowRules r = rules[blockIdx.y];
+  float* row = logits + (size_t)blockIdx.y * vocab;
   const unsigned* mask = r.mask_row >= 0 ? masks + (size_t)r.mask_row * words : nullptr;
-  __shared__ int found;
+  const int tid = threadIdx.x;
+  if (blockIdx.x > 0) {
+    if (mask == nullptr) return;
+    // quad q holds the logits 4 q - lead to 4 q - lead + 3: those that lie in one 16 bytes of memory
+    const int lead = (int)(((uintptr_t)row >> 2) & 3), count = (vocab + lead + 3) / 4;
+    const int q0 = (int)(blockIdx.x - 1) * (ADJUST_THREADS * ADJUST_AHEAD) + tid;
+    unsigned bits[ADJUST_AHEAD];
+#pragma unroll
+    for (int k = 0; k < ADJUST_AHEAD; ++k) {
+      const int i = min(max(4 * (q0 + k * ADJUST_THREADS) - lead, 0), vocab - 1), w = i >> 5;
+      const unsigned long long both = ((unsigned long long)mask[min(w + 1, words - 1)] << 32) | mask[w];     // (it may end in the next word)
+      bits[k] = (unsigned)(both >> (i & 31));
+    }
+#pragma unroll
+    for (int k = 0; k < ADJUST_AHEAD; ++k) {
+      const int q = q0 + k * ADJUST_THREADS, i = 4 * q - lead;
+      if (q >= count) continue;
+      if (i >= 0 && i + 3 < vocab && (bits[k] & 15u) == 0) {
+        *(f32x4*)(row + i) = f32x4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (i + e >= 0 && i + e < vocab && !((bits[k] >> (i < 0 ? i + e : e)) & 1u)) row[i + e] = -INFINITY;
+      }
+    }
+    return;
+  }
+  // the first of the biases are asked for now, to be there when the history is done
+  int bias_at = r.bias_begin + tid, bias_token = 0;
+  float bias = 0.f;
+  if (bias_at < r.bias_end) {
+    bias_token = bias_tokens[bias_at];
+    bias = bias_values[bias_at];
+  }
   if (r.slot >= 0) {
-    if (threadIdx.x == 0) found = 0;
-    __syncthreads();
+    __shared__ int found;
+    if (tid == 0) found = 0;
     int2* mine = entries + (size_t)r.slot * capacity;
     const int n = max(0, min(used[r.slot], capacity)), token = last[r.slot];
-    for (int i = threadIdx.x; i < n; i += 256) {
-      int2 e = mine[i];
-      if (e.x == token) {
-        e.y += 2;
-        mine[i].y = e.y;
-        found = 1;
+    __syncthreads();
+    for (int i0 = tid; i0 < n; i0 += ADJUST_THREADS * ADJUST_AHEAD) {
+      int2 e[ADJUST_AHEAD];
+      float x[ADJUST_AHEAD];
+      bool on[ADJUST_AHEAD];
+#pragma unroll
+      for (int k = 0; k < ADJUST_AHEAD; ++k) {
+        const int i = i0 + k * ADJUST_THREADS;
+        e[k] = i < n ? mine[i] : make_int2(-1, 0);
       }
-      if (e.x >= 0 && e.x < vocab && is_allowed(mask, e.x)) row[e.x] = penalised(row[e.x], r, e.y);
+#pragma unroll
+      for (int k = 0; k < ADJUST_AHEAD; ++k) {
+        const bool there = e[k].x >= 0 && e[k].x < vocab;
+        x[k] = there ? row[e[k].x] : 0.f;
+        on[k] = there && is_allowed(mask, e[k].x);
+      }
+#pragma unroll
+      for (int k = 0; k < ADJUST_AHEAD; ++k) {
+        const int i = i0 + k * ADJUST_THREADS;
+        if (i < n && e[k].x == token) {
+          e[k].y += 2;
+          mine[i].y = e[k].y;
+          found = 1;
+        }
+        if (on[k]) row[e[k].x] = penalised(x[k], r, e[k].y);
+      }
     }
     __syncthreads();
-    if (threadIdx.x == 0 && !found && token >= 0 && token < vocab && n < capacity) {
+    if (tid == 0 && !found && token >= 0 && token < vocab && n < capacity) {
       mine[n] = make_int2(token, 2);
       used[r.slot] = n + 1;
       if (is_allowed(mask, token)) row[token] = penalised(row[token], r, 2);
     }
     __syncthreads();
   }
-  for (int i = r.bias_begin + threadIdx.x; i < r.bias_end; i += 256) {
-    const int t = bias_tokens[i];
-    const float b = bias_values[i];
-    if (is_allowed(mask, t)) row[t] = b == -INFINITY ? b : row[t] + b;
+  while (bias_at < r.bias_end) {
+    if (is_allowed(mask, bias_token)) row[bias_token] = bias == -INFINITY ? bias : row[bias_token] + bias;
+    bias_at += ADJUST_THREADS;
+    if (bias_at < r.bias_end) {
+      bias_token = bias_tokens[bias_at];
+      bias = bias_values[bias_at];
+    }
   }
-  if (mask != nullptr)
-    for (int i = threadIdx.x; i < vocab; i += 256)
-      if (!is_allowed(mask, i)) row[i] = -INFINITY;
 }
 
 // The host has checked the rows' slots, masks and bias tokens against the sizes given here.
 extern "C" int tnx_adjust_logits(float* logits, const int* rules, const int* bias_tokens, const float* bias_values, int* entries, int* used,
                                  int capacity, const int* last, const int* masks, int rows, int vocab, hipStream_t stream) {
-  TNX_REQUIRE(rows >= 0 && vocab > 0 && capacity >= 0, "adjust_logits: bad sizes rows=%d vocab=%d capacity=%d", rows, vocab, capacity);
+  TNX_REQUIRE(rows >= 0 && rows <= 65535 && vocab > 0 && vocab < (1 << 30) && capacity >= 0,
+              "adjust_logits: bad sizes rows=%d vocab=%d capacity=%d", rows, vocab, capacity);
   if (rows == 0) return 0;
-  adjust_logits_kernel<<<rows, 256, 0, stream>>>(logits, (const RowRules*)rules, bias_tokens, bias_values, (int2*)entries, used, capacity,
-                                                 last, (const unsigned*)masks, (vocab + 31) / 32, vocab);
+  const int per_block = 4 * ADJUST_THREADS * ADJUST_AHEAD;
+  const int blocks = 1 + (masks ? (vocab + 3 + per_block - 1) / per_block : 0);
+  adjust_logits_kernel<<<dim3(blocks, rows), ADJUST_THREADS, 0, stream>>>(logits, (const RowRules*)rules, bias_tokens, bias_values,
+                                                                          (int2*)entries, used, capacity, last, (const unsigned*)masks,
+                                                                          (vocab + 31) / 32, vocab);
   TNX_CHECK_LAUNCH("adjust_logits");
   return 0;
 }
@@ -125,6 +187,12 @@ __device__ __forceinline__ unsigned long long order_key(float x, int idx) {
   return ((unsigned long long)u << 32) | (unsigned)(~(unsigned)idx);
 }
 
+// the logit of a key
+__device__ __forceinline__ float key_value(unsigned long long key) {
+  const unsigned u = (unsigned)(key >> 32);
+  return __uint_as_float((u & 0x80000000u) ? u & 0x7FFFFFFFu : ~u);
+}
+
 // exp(d) for d <= 0 by the hardware's power of two; log2(e) in two parts, so that only the roundings of d and of the power's argument
 // are left: 2^-24 of |d| each, and what is far below the largest adds little.
 __device__ __forceinline__ float exp_of(float d) {
@@ -140,11 +208,12 @@ struct Quads {
   __device__ __forceinline__ Quads(const float* r, int v)
       : row(r), vocab(v), lead((int)(((uintptr_t)r >> 2) & 3)), count((v + (int)(((uintptr_t)r >> 2) & 3) + 3) / 4) {}
   __device__ __forceinline__ int first(int q) const { return 4 * q - lead; }
+  template <bool ONCE = false>
   __device__ __forceinline__ f32x4 operator()(int q) const {
     const int i = 4 * q - lead;
     f32x4 x;
-    if (q < count && i >= 0 && i + 3 < vocab) {
-      x = *(const f32x4*)(row + i);
+    if (i >= 0 && i + 3 < vocab) {
+      x = ONCE ? __builtin_nontemporal_load((const f32x4*)(row + i)) : *(const f32x4*)(row + i);
     } else {
 #pragma unroll
       for (int e = 0; e < 4; ++e) x[e] = q < count && i + e >= 0 && i + e < vocab ? row[i + e] : -INFINITY;
@@ -155,10 +224,9 @@ struct Quads {
   }
 };
 
-#define SCORE_GROUPS 256       // groups of threads whose largest logits are ranked against one another
+#define SCORE_GROUPS 128       // groups of threads whose largest logits are ranked against one another
 #define SCORE_GATHER 1024      // the most logits that are gathered for the alternatives
 #define SCORE_MOST_TOP 32
-#define SCORE_WIDE_ROWS 512
 
 // One block of THREADS a row, one pass over it with a running maximum and sum.
 //
@@ -167,7 +235,7 @@ struct Quads {
 // the logits of these groups are looked at again, and those of them that are no smaller than the last group's best, hardly more than
 // the alternatives themselves, are ranked in LDS. Should they be more than fit (the best of a long row all in a few threads' places),
 // the alternatives are found one by one, each with a pass of its own.
-template <int THREADS, bool TOP>
+template <int THREADS, bool TOP, bool ONCE>
 __global__ void __launch_bounds__(THREADS)
 log_probs_kernel(const float* __restrict__ logits, const int* __restrict__ tokens, float* __restrict__ out, int* __restrict__ top_tokens,
                  float* __restrict__ top_out, int top, int vocab) {
@@ -178,11 +246,12 @@ log_probs_kernel(const float* __restrict__ logits, const int* __restrict__ token
   const float* row = quads.row;
 
   float m = -INFINITY, s = 0.f;
-  int at = tid;                       // the quads among which the thread's largest logit came first
+  int at = quads.first(tid);          // where the thread's largest logit came first
+  if (at < 0) at = 0;
   for (int q0 = tid; q0 < quads.count; q0 += 4 * THREADS) {
     f32x4 v[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] = quads(q0 + k * THREADS);
+    for (int k = 0; k < 4; ++k) v[k] = quads.template operator()<ONCE>(q0 + k * THREADS);
     float here = v[0][0];
 #pragma unroll
     for (int k = 0; k < 4; ++k)
@@ -191,7 +260,12 @@ log_probs_kernel(const float* __restrict__ logits, const int* __restrict__ token
     if (here > m) {
       s *= m > -INFINITY ? exp_of(m - here) : 0.f;
       m = here;
-      at = q0;
+      if constexpr (TOP) {
+#pragma unroll
+        for (int k = 3; k >= 0; --k)
+#pragma unroll
+          for (int e = 3; e >= 0; --e) at = v[k][e] == here ? quads.first(q0 + k * THREADS) + e : at;
+      }
     }
     const float base = fmaxf(m, -3.402823466e38f);       // -inf less -inf would be no number
 #pragma unroll
@@ -226,20 +300,7 @@ log_probs_kernel(const float* __restrict__ logits, const int* __restrict__ token
     __shared__ int winners[SCORE_MOST_TOP], num_winners, num_gathered;
     __shared__ unsigned long long least;
     // the thread's best as a key (its logit, then the lower token id), and its group's
-    unsigned long long key = 0;
-    if (tid < quads.count) {
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const f32x4 x = quads(at + k * THREADS);
-        const int i = quads.first(at + k * THREADS);
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (i + e >= 0 && i + e < vocab) {
-            const unsigned long long other = order_key(x[e], i + e);
-            key = other > key ? other : key;
-          }
-      }
-    }
+    unsigned long long key = tid < quads.count ? order_key(mine, at) : 0;
 #pragma unroll
     for (int o = 1; o < PER_GROUP; o <<= 1) {
       const unsigned long long other = __shfl_xor(key, o, 64);
@@ -292,7 +353,7 @@ log_probs_kernel(const float* __restrict__ logits, const int* __restrict__ token
         if (rank < top) {
           const int t = (int)(~(unsigned)k);
           ids[rank] = t;
-          values[rank] = log_prob_of(row[t], m, log_l);
+          values[rank] = log_prob_of(key_value(k), m, log_l);
         }
       }
     } else {
@@ -316,18 +377,18 @@ log_probs_kernel(const float* __restrict__ logits, const int* __restrict__ token
         if (tid == 0) {
           const int t = (int)(~(unsigned)b);
           ids[r] = t;
-          values[r] = log_prob_of(row[t], m, log_l);
+          values[r] = log_prob_of(key_value(b), m, log_l);
         }
       }
     }
   }
 }
 
-template <int THREADS>
+template <int THREADS, bool ONCE>
 static void launch_log_probs(const float* logits, const int* tokens, float* out, int* top_tokens, float* top_out, int top, int rows, int vocab,
                              hipStream_t stream) {
-  if (top) log_probs_kernel<THREADS, true><<<rows, THREADS, 0, stream>>>(logits, tokens, out, top_tokens, top_out, top, vocab);
-  else log_probs_kernel<THREADS, false><<<rows, THREADS, 0, stream>>>(logits, tokens, out, top_tokens, top_out, top, vocab);
+  if (top) log_probs_kernel<THREADS, true, ONCE><<<rows, THREADS, 0, stream>>>(logits, tokens, out, top_tokens, top_out, top, vocab);
+  else log_probs_kernel<THREADS, false, ONCE><<<rows, THREADS, 0, stream>>>(logits, tokens, out, top_tokens, top_out, top, vocab);
 }
 
 extern "C" int tnx_log_probs(const float* logits, const int* tokens, float* out, int* top_tokens, float* top_out, int top, int rows,
@@ -335,8 +396,15 @@ extern "C" int tnx_log_probs(const float* logits, const int* tokens, float* out,
   TNX_REQUIRE(rows >= 0 && vocab > 0 && vocab < (1 << 30) && top >= 0 && top <= SCORE_MOST_TOP && top <= vocab,
               "log_probs: bad sizes rows=%d vocab=%d top=%d", rows, vocab, top);
   if (rows == 0) return 0;
-  if (rows <= SCORE_WIDE_ROWS) launch_log_probs<1024>(logits, tokens, out, top_tokens, top_out, top, rows, vocab, stream);
-  else launch_log_probs<256>(logits, tokens, out, top_tokens, top_out, top, rows, vocab, stream);
+  // 1,024 threads where each has a whole round of 16 logits and the rows are no more than the blocks that run at once, 512 otherwise.
+  // In us, 1,024 / 512 / 256 threads: 64 rows of 50,272 with 20 alternatives 13.9 / 18.9 / 29.7, 512 rows 25.4 / 28.4 / 42.7, 777 rows
+  // 45.5 / 39.4 / 51.2; 64 rows of 5,000 with 5 7.1 / 6.4 / 7.5, 2,048 rows 29.4 / 18.3 / 18.0.
+  // Rows that the caches cannot hold are marked as read once: 2,048 rows of 50,272 without alternatives 65.8 us (6.3 TB/s), 73.5 plain,
+  // 2,048 of 32,001 44.0 and 48.4; but 777 of 32,001 (99 MB) with 20 27.6 and 26.1, 64 of 50,272 10.6 and 8.6.
+  const bool once = (long long)rows * vocab * 4 >= (128ll << 20);
+  if (rows <= 512 && vocab >= 16 * 1024) launch_log_probs<1024, false>(logits, tokens, out, top_tokens, top_out, top, rows, vocab, stream);
+  else if (once) launch_log_probs<512, true>(logits, tokens, out, top_tokens, top_out, top, rows, vocab, stream);
+  else launch_log_probs<512, false>(logits, tokens, out, top_tokens, top_out, top, rows, vocab, stream);
   TNX_CHECK_LAUNCH("log_probs");
   return 0;
 }
