@@ -71,8 +71,9 @@ class CacheManager:
     """
 
     def __init__(self, needs: Dict[int, CacheNeed], page_size: int, num_pages, max_seqs: int,
-                 dtype: torch.dtype, device, allocate: bool = True, page_pad_bytes: int = 0):
-        """`page_pad_bytes`: memory left between one page and the next in every page tensor (a multiple of 32).
+                 dtype: torch.dtype, device, allocate: bool = True, page_pad_bytes: int = 0, ops=None):
+        """`ops`: the kernel backend, which copies pages and state where requests are forked, pages moved.
+        `page_pad_bytes`: memory left between one page and the next in every page tensor (a multiple of 32).
         Pages whose size is a power of two lie at distances that are powers of two, and so do the requests
         that fill them side by side: the kernels that read all requests at once then meet the same memory
         channels at the same time. A few hundred bytes between pages take that regularity away."""
@@ -80,6 +81,9 @@ class CacheManager:
         if page_pad_bytes < 0 or page_pad_bytes % 32:
             raise ValueError(f"page_pad_bytes must be a multiple of 32 from 0 up, got {page_pad_bytes}")
         self.page_pad_bytes = page_pad_bytes
+        self.ops, self.needs, self.allocated = ops, dict(needs), allocate
+        self._row_sets: Dict[str, Dict[bool, object]] = {}     # group -> {bounded by tokens: the rows its pages are}
+        self._state_rows = None                             # the slots' rows, of every state tensor
         self.slots = SlotPool(max_seqs)
         self.groups: Dict[str, PageGroup] = {}
         self.caches: Dict[int, LayerCache] = {}
@@ -101,12 +105,7 @@ class CacheManager:
                 g.cache_ids.append(cid)
                 lc = LayerCache(cid, g.name)
                 if allocate:
-                    item = torch.empty(0, dtype=dtype).element_size()
-                    for name, shape in need.tensors_of_a_page():
-                        dims = [page_size if d == "page" else d for d in shape]
-                        count = int(np.prod(dims))
-                        whole = torch.empty(g.pool.num_pages, count + page_pad_bytes // item, dtype=dtype, device=device)
-                        lc.pages[name] = whole[:, :count].view(g.pool.num_pages, *dims)
+                    lc.pages.update(self._new_pages(need, g.pool.num_pages))
                     sdt = getattr(torch, need.state_dtype)
                     for name, shape in need.state_shapes:       # a mixer that keeps pages and a fixed state
                         lc.state[name] = torch.zeros(max_seqs, *shape, dtype=sdt, device=device)
@@ -120,6 +119,16 @@ class CacheManager:
                 self.caches[cid] = lc
             else:
                 raise ValueError(f"unknown cache kind {need.kind!r}")
+
+    def _new_pages(self, need: CacheNeed, num_pages: int) -> Dict[str, torch.Tensor]:
+        item = torch.empty(0, dtype=self.dtype).element_size()
+        out = {}
+        for name, shape in need.tensors_of_a_page():
+            dims = [self.page_size if d == "page" else d for d in shape]
+            count = int(np.prod(dims))
+            whole = torch.empty(num_pages, count + self.page_pad_bytes // item, dtype=self.dtype, device=self.device)
+            out[name] = whole[:, :count].view(num_pages, *dims)
+        return out
 
     # ---------------------------------------------------------------- sizes
 
@@ -204,6 +213,157 @@ class CacheManager:
             g.pool.free([p for p in r.tables[g.name] if p >= 0], req)
         self.slots.free(r.slot, req)
 
+    # ---------------------------------------------------------------- forks
+
+    # Bytes of a run of places of which a part is worth copying alone. Values turned inside a page lie in runs of a line or two of memory:
+    # a part of such a line costs more than the whole (24 pages of 40 of 64 tokens' values in all layers of OPT-6.7b 168 us, whole 91).
+    BOUNDED_RUN = 1024
+
+    def _rows(self, group: str, bounded: bool):
+        """What the pages of a group are to `copy_rows`, of every layer's tensors; `bounded`: with the axes that tokens are counted on."""
+        sets = self._row_sets.setdefault(group, {})
+        if bounded not in sets:
+            tensors, axes = [], []
+            for cid in self.groups[group].cache_ids:
+                for name, shape in self.needs[cid].tensors_of_a_page():
+                    t = self.caches[cid].pages[name]
+                    axis = 1 + tuple(shape).index("page") if "page" in shape else None
+                    run = 0 if axis is None else t.stride(axis) * t.shape[axis] * t.element_size()
+                    tensors.append(t)
+                    axes.append(axis if bounded and run >= self.BOUNDED_RUN else None)
+            sets[bounded] = self.ops.row_set(tensors, axes)
+        return sets[bounded]
+
+    def _state_tensors(self) -> List[torch.Tensor]:
+        return [t for lc in self.caches.values() if lc.writes for t in lc.state.values()]
+
+    def _copier(self):
+        if self.ops is None:
+            raise RuntimeError("this cache was made without a kernel backend and cannot copy what it holds")
+        return self.ops
+
+    @property
+    def has_state(self) -> bool:
+        return any(n is not None and bool(n.state_shapes) for n in self.needs.values())
+
+    def can_fork(self, parent: Hashable, num_tokens: int) -> bool:
+        """Whether the first `num_tokens` tokens of `parent` can be taken over: fixed state is that of the newest token alone, and
+        of a windowed group the pages that a later query reads must not have been given back."""
+        if parent not in self.requests:
+            return False
+        r = self.requests[parent]
+        if not 0 <= num_tokens <= r.num_tokens or (self.has_state and num_tokens != r.num_tokens):
+            return False
+        for g in self.groups.values():
+            table = r.tables[g.name]
+            if any(table[b] < 0 for b in range(self._first_block(g, num_tokens), self._blocks_for(num_tokens))):
+                return False
+        return True
+
+    def _first_block(self, g: PageGroup, num_tokens: int) -> int:
+        """The first block that queries at `num_tokens` and later read (see `advance`)."""
+        return 0 if g.window is None else max(0, num_tokens - g.window + 1) // self.page_size
+
+    def fork(self, parent: Hashable, child: Hashable, num_tokens: Optional[int] = None) -> int:
+        """`child` becomes a request that holds the first `num_tokens` tokens of `parent` (all it holds, if not given), without computing
+        them: full pages are shared, each request keeps them until both have given them back; the page that is not full, which both will
+        write to, and the fixed state are copied, by launches on the current stream. All it needs, or nothing, is taken. Returns its slot."""
+        r = self.requests[parent]
+        n = r.num_tokens if num_tokens is None else int(num_tokens)
+        if child in self.requests:
+            raise ValueError(f"request {child!r} is already live")
+        if not self.can_fork(parent, n):
+            raise ValueError(f"request {parent!r} holds {r.num_tokens} tokens, of which the first {n} cannot be taken over")
+        full, rest = divmod(n, self.page_size)
+        if rest:
+            for g in self.groups.values():
+                if g.pool.num_free < 1:
+                    raise OutOfPages(f"group {g.name}: a page wanted for request {child!r}, none free")
+        if self.allocated and (rest and self.groups or self.has_state):
+            self._copier()
+        slot = self.slots.allocate(child)
+        mine = self.requests[child] = RequestPages(slot, n, {name: [] for name in self.groups})
+        try:
+            for g in self.groups.values():
+                first, theirs, table = self._first_block(g, n), r.tables[g.name], mine.tables[g.name]
+                shared = theirs[first:full]
+                g.pool.share(shared, child)
+                table += [-1] * min(first, full) + shared
+                if rest:
+                    table += g.pool.allocate(1, child)
+                    if self.allocated:
+                        rows = self._rows(g.name, True)
+                        self.ops.copy_rows(rows, [theirs[full]], [table[-1]], [rest] if rows.places is not None else None)
+            if self.allocated and self.has_state:
+                if self._state_rows is None:
+                    self._state_rows = self.ops.row_set(self._state_tensors())
+                self.ops.copy_rows(self._state_rows, [r.slot], [slot])
+        except Exception:
+            self.free_request(child)
+            raise
+        return slot
+
+    def rename(self, req: Hashable, name: Hashable) -> None:
+        """The request goes by another name from now on."""
+        if name in self.requests:
+            raise ValueError(f"request {name!r} is already live")
+        r = self.requests.pop(req)
+        for g in self.groups.values():
+            g.pool.rename([p for p in r.tables[g.name] if p >= 0], req, name)
+        self.slots.rename(r.slot, req, name)
+        self.requests[name] = r
+
+    # ---------------------------------------------------------------- where pages lie
+
+    def _renumber(self, g: PageGroup, where: Dict[int, int]) -> None:
+        for r in self.requests.values():
+            r.tables[g.name] = [where[p] if p >= 0 else -1 for p in r.tables[g.name]]
+
+    def compact(self) -> int:
+        """Held pages move to the lowest numbers of their pools (one launch a group, on the current stream); the number moved. Requests
+        keep what they hold; block tables made before are void."""
+        moved = 0
+        for g in self.groups.values():
+            where = g.pool.packed(g.pool.num_pages)
+            moves = [(p, q) for p, q in where.items() if p != q]
+            if not moves:
+                continue
+            if self.allocated:
+                self._copier().copy_rows(self._rows(g.name, False), [p for p, _ in moves], [q for _, q in moves])
+            g.pool.repack(where, g.pool.num_pages)
+            self._renumber(g, where)
+            moved += len(moves)
+        return moved
+
+    def resize(self, num_pages) -> None:
+        """Pools of another size (an int for all groups, or {group name: int}), with what is held carried over, layer by layer, so that
+        one layer at a time lies in memory twice. `OutOfPages`, and nothing changed, where more pages are held than asked for."""
+        sizes = {name: num_pages[name] if isinstance(num_pages, dict) else num_pages for name in self.groups}
+        if any(n <= 0 for n in sizes.values()):
+            raise ValueError(f"a page pool needs at least one page, got {num_pages}")
+        for name, g in self.groups.items():
+            g.pool.packed(sizes[name])               # (raises where they do not fit)
+        if self.allocated and self.groups:
+            self._copier()
+        self.compact()
+        # From here on a page keeps its number, so a layer that has its new tensors and one that has its old ones go by the same tables:
+        # where memory runs out in between, the pools are as large as the smaller of the two, and all is as it was.
+        self._row_sets.clear()
+        for name, g in self.groups.items():
+            held = [p for p in range(g.pool.num_pages) if g.pool.holders_of(p)]
+            where = {p: p for p in held}
+            try:
+                for cid in g.cache_ids if self.allocated else ():
+                    lc = self.caches[cid]
+                    new = self._new_pages(self.needs[cid], sizes[name])
+                    if held:
+                        self.ops.copy_rows(self.ops.row_set([lc.pages[k] for k in new], targets=list(new.values())), held, held)
+                    lc.pages.update(new)             # (the dictionary is the readers' too)
+            except Exception:
+                g.pool.repack(where, min(sizes[name], g.pool.num_pages))
+                raise
+            g.pool.repack(where, sizes[name])
+
     def reset(self) -> None:
         for req in list(self.requests):
             self.free_request(req)
@@ -223,18 +383,19 @@ class CacheManager:
         return out
 
     def check(self) -> None:
-        """No page lost, none held twice; tables agree with the pools."""
+        """No page lost, none in a table whose request does not hold it; tables agree with the pools."""
         for g in self.groups.values():
             g.pool.check()
-            seen = set()
+            holders: Dict[int, set] = {}
             for req, r in self.requests.items():
                 for p in r.tables[g.name]:
                     if p < 0:
                         continue
-                    if p in seen:
-                        raise AssertionError(f"page {p} of group {g.name} is in two tables")
-                    seen.add(p)
-                    if g.pool.holder_of(p) != req:
-                        raise AssertionError(f"page {p} is in {req!r}'s table but held by {g.pool.holder_of(p)!r}")
-            if len(seen) + g.pool.num_free != g.pool.num_pages:
-                raise AssertionError(f"group {g.name}: {g.pool.num_pages - len(seen) - g.pool.num_free} pages lost")
+                    if req in holders.setdefault(p, set()):
+                        raise AssertionError(f"page {p} of group {g.name} is twice in {req!r}'s table")
+                    holders[p].add(req)
+            for p, reqs in holders.items():
+                if set(g.pool.holders_of(p)) != reqs:
+                    raise AssertionError(f"page {p} is in the tables of {reqs!r} but held by {g.pool.holders_of(p)!r}")
+            if len(holders) + g.pool.num_free != g.pool.num_pages:
+                raise AssertionError(f"group {g.name}: {g.pool.num_pages - len(holders) - g.pool.num_free} pages lost")

@@ -55,10 +55,11 @@ __device__ __forceinline__ float penalised(float x, const RowRules& r, int info)
 }
 
 #define ADJUST_THREADS 1024
-#define ADJUST_AHEAD 4         // history entries (or quads of barred tokens) of a thread that are on their way together
+#define ADJUST_AHEAD 4         // history entries of a thread that are on their way together
+#define ADJUST_BARRED 16       // logits that a thread may have to bar
 
 // Block 0 of a row does what names single tokens, its history and its biases; the others write -inf where the mask bars a token,
-// ADJUST_THREADS * ADJUST_AHEAD quads of logits each. A logit is written by one thread at a time: history entries name distinct tokens,
+// ADJUST_THREADS * ADJUST_BARRED logits each. A logit is written by one thread at a time: history entries name distinct tokens,
 // so do a row's biases, a barrier lies between the two, and barred tokens are left to the other blocks, which write nothing else.
 //
 // Of a row's logits only those named are read, and only those barred written: what bounds a batch without masks is the way from the
@@ -73,27 +74,14 @@ adjust_logits_kernel(float* __restrict__ logits, const RowRules* __restrict__ ru
   const int tid = threadIdx.x;
   if (blockIdx.x > 0) {
     if (mask == nullptr) return;
-    // quad q holds the logits 4 q - lead to 4 q - lead + 3: those that lie in one 16 bytes of memory
-    const int lead = (int)(((uintptr_t)row >> 2) & 3), count = (vocab + lead + 3) / 4;
-    const int q0 = (int)(blockIdx.x - 1) * (ADJUST_THREADS * ADJUST_AHEAD) + tid;
-    unsigned bits[ADJUST_AHEAD];
+    const int i0 = (int)(blockIdx.x - 1) * (ADJUST_THREADS * ADJUST_BARRED) + tid;
+    unsigned word[ADJUST_BARRED];
 #pragma unroll
-    for (int k = 0; k < ADJUST_AHEAD; ++k) {
-      const int i = min(max(4 * (q0 + k * ADJUST_THREADS) - lead, 0), vocab - 1), w = i >> 5;
-      const unsigned long long both = ((unsigned long long)mask[min(w + 1, words - 1)] << 32) | mask[w];     // (it may end in the next word)
-      bits[k] = (unsigned)(both >> (i & 31));
-    }
+    for (int k = 0; k < ADJUST_BARRED; ++k) word[k] = mask[min(i0 + k * ADJUST_THREADS, vocab - 1) >> 5];
 #pragma unroll
-    for (int k = 0; k < ADJUST_AHEAD; ++k) {
-      const int q = q0 + k * ADJUST_THREADS, i = 4 * q - lead;
-      if (q >= count) continue;
-      if (i >= 0 && i + 3 < vocab && (bits[k] & 15u) == 0) {
-        *(f32x4*)(row + i) = f32x4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (i + e >= 0 && i + e < vocab && !((bits[k] >> (i < 0 ? i + e : e)) & 1u)) row[i + e] = -INFINITY;
-      }
+    for (int k = 0; k < ADJUST_BARRED; ++k) {
+      const int i = i0 + k * ADJUST_THREADS;
+      if (i < vocab && !((word[k] >> (i & 31)) & 1u)) row[i] = -INFINITY;
     }
     return;
   }
@@ -160,8 +148,8 @@ extern "C" int tnx_adjust_logits(float* logits, const int* rules, const int* bia
   TNX_REQUIRE(rows >= 0 && rows <= 65535 && vocab > 0 && vocab < (1 << 30) && capacity >= 0,
               "adjust_logits: bad sizes rows=%d vocab=%d capacity=%d", rows, vocab, capacity);
   if (rows == 0) return 0;
-  const int per_block = 4 * ADJUST_THREADS * ADJUST_AHEAD;
-  const int blocks = 1 + (masks ? (vocab + 3 + per_block - 1) / per_block : 0);
+  const int per_block = ADJUST_THREADS * ADJUST_BARRED;
+  const int blocks = 1 + (masks ? (vocab + per_block - 1) / per_block : 0);
   adjust_logits_kernel<<<dim3(blocks, rows), ADJUST_THREADS, 0, stream>>>(logits, (const RowRules*)rules, bias_tokens, bias_values,
                                                                           (int2*)entries, used, capacity, last, (const unsigned*)masks,
                                                                           (vocab + 31) / 32, vocab);

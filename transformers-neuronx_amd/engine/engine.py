@@ -13,7 +13,8 @@ import torch
 from ..config.engine_config import EngineConfig
 from ..kernels import LostStep
 from ..sampling.params import SamplingParams
-from ..sampling.sampler import Sampler
+from ..kernels.steering import pack_mask
+from ..sampling.sampler import Sampler, Steering, banned_ngram_tokens
 from .batch import StepEntry
 from .runner import ModelRunner
 from .scheduler import PENDING, Request, ScheduledRun, Scheduler
@@ -25,6 +26,9 @@ class StepOutput:
     token: int
     finished: bool
     finish_reason: Optional[str]
+    # of a request that asks for them (`SamplingParams.logprobs`): the token's log-probability, and (token, its own) of the largest logits
+    logprob: Optional[float] = None
+    top_logprobs: Optional[list] = None
 
 
 @dataclass
@@ -34,6 +38,7 @@ class _StartedStep:
     sampling: List[ScheduledRun]
     sent: object                         # the tokens on their way to the host (`ops.send_tokens`)
     started: float
+    scores: object = None                # the tokens' log-probabilities on their way (`ops.send_log_probs`), where asked for
 
 
 class LLMEngine:
@@ -49,7 +54,8 @@ class LLMEngine:
         max_len = min(config.max_model_len or runner.max_positions, runner.max_positions)
         self.scheduler = Scheduler(runner.cache, config.max_num_seqs, config.max_num_batched_tokens, max_len,
                                    max_portion=config.chunk_size, prompts_first=config.prompts_first)
-        self.sampler = Sampler(runner.ops, runner.model.device)
+        self.sampler = Sampler(runner.ops, runner.model.device, slots=runner.cache.max_seqs, capacity=min(runner.vocab, max_len + 1),
+                               last=runner.kept_tokens)
         self.requests: Dict[Hashable, Request] = {}
         self._ids = itertools.count()
         self._taken = 0                        # requests taken since the start or the last reset
@@ -66,20 +72,86 @@ class LLMEngine:
     def add_request(self, prompt: Sequence[int], params: SamplingParams, req_id: Optional[Hashable] = None):
         if params.max_new_tokens < 1:
             raise ValueError("max_new_tokens must be at least 1")
+        return self._add(prompt, params, req_id)
+
+    def _add(self, prompt: Sequence[int], params: SamplingParams, req_id: Optional[Hashable], leader: Optional[Request] = None,
+             output: Sequence[int] = ()):
         rid = req_id if req_id is not None else next(self._ids)
         if rid in self.requests and not self.requests[rid].finished:
             raise ValueError(f"request {rid!r} is already live")
         prompt = [int(t) for t in prompt]
-        if prompt and not 0 <= min(prompt) <= max(prompt) < self.runner.vocab:
-            raise ValueError(f"request {rid!r}: a token id of the prompt is outside the vocabulary of {self.runner.vocab}")
+        vocab = self.runner.vocab
+        if prompt and not 0 <= min(prompt) <= max(prompt) < vocab:
+            raise ValueError(f"request {rid!r}: a token id of the prompt is outside the vocabulary of {vocab}")
+        if params.biases and not 0 <= params.biases[0][0] <= params.biases[-1][0] < vocab:
+            raise ValueError(f"request {rid!r}: a logit bias names a token outside the vocabulary of {vocab}")
         if params.seed is None:
             # a stream of the request's own, the same whatever else runs beside it
             params = dataclasses.replace(params, seed=int(self.config.seed) + self._taken)
-        self._taken += 1
-        req = Request(rid, prompt, params)
+        req = Request(rid, prompt, params, output=list(output), leader=leader)
+        req.mask = self._mask(req)
+        if req.mask is not None and not req.mask.any():
+            raise ValueError(f"request {rid!r}: no token is allowed")
         self.scheduler.add(req)
+        self._taken += 1
         self.requests[rid] = req
         return rid
+
+    def add_samples(self, prompt: Sequence[int], params: SamplingParams, count: int, req_id: Optional[Hashable] = None) -> List[Hashable]:
+        """`count` requests for one prompt, each with a random stream of its own (the seeds that follow `params.seed`). The prompt is
+        computed once, by the first of them, all but its newest token; the others take its pages over, where they are admitted while
+        it still runs. Their names: `req_id`, (`req_id`, 1), (`req_id`, 2) and so on."""
+        if count < 1:
+            raise ValueError(f"at least one sample is wanted, got {count}")
+        if params.max_new_tokens < 1:
+            raise ValueError("max_new_tokens must be at least 1")
+        rid = req_id if req_id is not None else next(self._ids)
+        names = [rid] + [(rid, i) for i in range(1, count)]
+        for name in names:
+            if name in self.requests and not self.requests[name].finished:
+                raise ValueError(f"request {name!r} is already live")
+        streams = [params] + [params if params.seed is None else dataclasses.replace(params, seed=params.seed + i) for i in range(1, count)]
+        self._add(prompt, streams[0], names[0])
+        for name, stream in zip(names[1:], streams[1:]):
+            self._add(prompt, stream, name, leader=self.requests[rid])
+        return names
+
+    def fork_request(self, req_id: Hashable, params: Optional[SamplingParams] = None, new_id: Optional[Hashable] = None) -> Hashable:
+        """Another request that goes on from where `req_id` stands, with its prompt and the tokens that have been reported of it, by
+        `params` (its own with the seed that follows, if not given; `max_new_tokens` counts the tokens taken over too). It shares the
+        pages of the tokens it has in common while `req_id` runs; where it cannot, they are computed again. Its name is returned."""
+        req = self.requests[req_id]
+        output = req.output[:req.output.index(PENDING)] if PENDING in req.output else list(req.output)
+        if params is None:
+            params = dataclasses.replace(req.params, seed=(req.params.seed or 0) + 1)
+        if params.max_new_tokens <= len(output):
+            raise ValueError(f"request {req_id!r} has {len(output)} tokens already, max_new_tokens is {params.max_new_tokens}")
+        child = self._add(req.prompt, params, new_id, leader=None if req.finished else req, output=output)
+        if params.logprobs is not None:
+            # of the tokens taken over, what is known of them
+            q = self.requests[child]
+            known = len(output) if len(req.logprobs) >= len(output) else 0
+            q.logprobs = req.logprobs[:known] + [0.0] * (len(output) - known)
+            q.top_logprobs = req.top_logprobs[:known] + [[] for _ in range(len(output) - known)]
+        return child
+
+    def resize_cache(self, num_pages) -> None:
+        """Another number of cache pages, between two steps; live requests keep theirs (`ModelRunner.resize_cache`)."""
+        self.runner.resize_cache(num_pages)
+
+    def _mask(self, req: Request):
+        """The tokens that may come next, where the request says which: those it allows but for those barred otherwise."""
+        p = req.params
+        if p.allowed_tokens is None:
+            return None
+        vocab = self.runner.vocab
+        words = pack_mask(vocab, p.allowed_tokens(list(req.output)) if p.follows_grammar else p.allowed_tokens)
+        barred = [t for t, b in p.biases if b == float("-inf")] + (list(p.eos_ids) if p.ban_eos else [])
+        if p.no_repeat_ngram_size:
+            barred += banned_ngram_tokens(req.prompt + req.output, p.no_repeat_ngram_size)
+        if barred:
+            words &= ~pack_mask(vocab, [t for t in set(barred) if 0 <= t < vocab])
+        return words
 
     @property
     def has_work(self) -> bool:
@@ -103,7 +175,7 @@ class LLMEngine:
             entries.append(StepEntry(run.request.req_id, toks, [run.count - 1] if run.samples else []))
         logits = self.runner.step(entries, kept_allowed=True)
         sampling = [r for r in runs if r.samples]
-        sent = None
+        sent = scores = None
         if sampling:
             requests = [r.request for r in sampling]
             if self.logits_hook is not None:
@@ -114,10 +186,31 @@ class LLMEngine:
                 histories = [list(q.prompt) + list(q.output) if q.params.no_repeat_ngram_size else None
                              for q in requests]
             drawn = self.sampler.draw(logits, [q.params for q in requests], [len(q.output) for q in requests],
-                                      histories)
+                                      histories, self._steering(requests))
+            tops = [q.params.logprobs for q in requests if q.params.logprobs is not None]
+            if tops:
+                scores = self.runner.ops.send_log_probs(*self.runner.ops.log_probs(logits, drawn, min(max(tops), logits.shape[1])))
             sent = self.runner.keep_tokens(drawn)
         self.scheduler.record(runs)
-        return _StartedStep(runs, sampling, sent, t0)
+        return _StartedStep(runs, sampling, sent, t0, scores)
+
+    def _steering(self, requests: List[Request]) -> Optional[List[Optional[Steering]]]:
+        if not any(q.mask is not None or q.params.penalised for q in requests):
+            return None
+        out: List[Optional[Steering]] = []
+        for q in requests:
+            steering = None
+            if q.mask is not None or q.params.penalised:
+                slot = self.runner.cache.slot_of(q.req_id)
+                steering = Steering(slot, mask=q.mask)
+                # the device goes on with the history it has, but for a request that was just admitted, or admitted again
+                if q.params.penalised and q.history_of != (slot, q.preemptions):
+                    if PENDING in q.output:
+                        raise AssertionError(f"request {q.req_id!r} was admitted with a token that is not known yet")
+                    steering.start = (q.prompt, list(q.output))
+                    q.history_of = (slot, q.preemptions)
+            out.append(steering)
+        return out
 
     def _finish(self, step: _StartedStep) -> List[StepOutput]:
         """Read the tokens of a started step and give them to their requests."""
@@ -126,6 +219,21 @@ class LLMEngine:
             it = iter(self.runner.receive_tokens(step.sent))
             tokens = [next(it) if r.samples else None for r in step.runs]
         kept = self.scheduler.resolve(step.runs, tokens)
+        if step.scores is not None:
+            log_probs, ids, best = self.runner.ops.receive_log_probs(step.scores)
+            at = 0
+            for r, t in zip(step.runs, kept):
+                if t is not None and r.request.params.logprobs is not None:
+                    top = r.request.params.logprobs
+                    r.request.logprobs.append(log_probs[at])
+                    r.request.top_logprobs.append(list(zip(ids[at][:top], best[at][:top])) if top else [])
+                at += r.samples
+        for r, t in zip(step.runs, kept):
+            q = r.request
+            if t is not None and not q.finished and q.mask is not None and (q.params.follows_grammar or q.params.no_repeat_ngram_size):
+                q.mask = self._mask(q)
+                if not q.mask.any():
+                    self.scheduler._end(q, "grammar", [])
         self.scheduler.finished.clear()        # the engine reports ends through `StepOutput`; nothing piles up
         if self.record_timings:
             self.runner.ops.synchronize()
@@ -138,7 +246,9 @@ class LLMEngine:
             if t is not None:
                 q = r.request
                 last = q.finished and r.out_index == len(q.output) - 1
-                out.append(StepOutput(q.req_id, t, last, q.finish_reason if last else None))
+                scored = q.params.logprobs is not None
+                out.append(StepOutput(q.req_id, t, last, q.finish_reason if last else None,
+                                      q.logprobs[r.out_index] if scored else None, q.top_logprobs[r.out_index] if scored else None))
         return out
 
     @torch.no_grad()
@@ -153,8 +263,8 @@ class LLMEngine:
             raise
 
     def _step(self) -> List[StepOutput]:
-        # a request that may not repeat its n-grams needs its last token on the host before the next is chosen
-        in_step = any(q.params.no_repeat_ngram_size and not q.finished for q in self.requests.values())
+        # a request that may not repeat its n-grams, or follows a grammar, needs its last token on the host before the next is chosen
+        in_step = any((q.params.no_repeat_ngram_size or q.params.follows_grammar) and not q.finished for q in self.requests.values())
         idle = self._started is None
         if not self.run_ahead or self.record_timings or in_step:
             out = self._finish(self._started) if self._started is not None else []
@@ -201,13 +311,30 @@ class LLMEngine:
                 if on_token:
                     on_token(out)
 
-    def generate(self, prompts: Sequence[Sequence[int]], params) -> List[List[int]]:
+    def generate(self, prompts: Sequence[Sequence[int]], params, samples: int = 1, best_of: Optional[int] = None) -> List[List[int]]:
         """Generated tokens (without the prompts) of a set of prompts; `params` is one
-        `SamplingParams` for all or a list with one each."""
+        `SamplingParams` for all or a list with one each. `samples` answers to each prompt, one behind the other (`add_samples`); with
+        `best_of`, so many are made and those kept whose tokens have the largest sum of log-probabilities, largest first."""
+        return [list(q.output) for family in self.generate_requests(prompts, params, samples, best_of) for q in family]
+
+    def generate_requests(self, prompts: Sequence[Sequence[int]], params, samples: int = 1,
+                          best_of: Optional[int] = None) -> List[List[Request]]:
+        """The same as requests that have ended, `samples` a prompt."""
         plist = params if isinstance(params, (list, tuple)) else [params] * len(prompts)
-        ids = [self.add_request(p, sp) for p, sp in zip(prompts, plist)]
+        made = samples if best_of is None else best_of
+        if samples < 1 or made < samples:
+            raise ValueError(f"{samples} samples, at least one and no more than best_of ({best_of}), are wanted")
+        if made > samples:
+            plist = [sp if sp.logprobs is not None else dataclasses.replace(sp, logprobs=0) for sp in plist]
+        families = [self.add_samples(p, sp, made) if made > 1 else [self.add_request(p, sp)] for p, sp in zip(prompts, plist)]
         self.run()
-        return [list(self.pop_request(i).output) for i in ids]
+        out = []
+        for names in families:
+            family = [self.pop_request(name) for name in names]
+            if made > samples:
+                family = sorted(family, key=lambda q: -q.cumulative_logprob)[:samples]     # (of equal ones the earlier)
+            out.append(family)
+        return out
 
     def abort_request(self, req_id: Hashable) -> Request:
         """Stop a request whose caller has gone, between two calls of `step()`: its pages and its slot are

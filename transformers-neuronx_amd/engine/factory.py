@@ -88,7 +88,7 @@ def build_runner(model_config, source, cfg: EngineConfig) -> ModelRunner:
         model.finish_load()
         torch.cuda.empty_cache()
     num_pages = size_page_pool(cfg, bytes_per_page, device)
-    cache = CacheManager(needs, cfg.page_size, num_pages, cfg.max_num_seqs, cfg.dtype, device, page_pad_bytes=pad)
+    cache = CacheManager(needs, cfg.page_size, num_pages, cfg.max_num_seqs, cfg.dtype, device, page_pad_bytes=pad, ops=ops)
     return ModelRunner(model, cache, ops, use_graphs=cfg.use_graphs)
 
 

@@ -17,6 +17,7 @@ import torch
 import numpy as np
 
 from ..cache.manager import CacheManager
+from ..cache.pages import OutOfPages
 from .. import debug
 from ..kernels import LostStep
 from .batch import PackedStep, StepContext, StepEntry, context_from, pack_step
@@ -228,6 +229,57 @@ class ModelRunner:
         tokens = self.ops.receive_tokens(sent)
         self.raise_if_lost()
         return tokens
+
+    # ---------------------------------------------------------------- several requests from one
+
+    def fork(self, parent: Hashable, child: Hashable, num_tokens: Optional[int] = None) -> None:
+        """`child` goes on from the first `num_tokens` tokens of `parent` (all it holds, if not given): see `CacheManager.fork`."""
+        self.raise_if_lost()
+        self.cache.fork(parent, child, num_tokens)
+
+    def reorder(self, names: List[Hashable], parents: List[int]) -> None:
+        """Request `names[i]` becomes what `names[parents[i]]` holds now, as a search over beams wants it after each choice: one that
+        nobody goes on from is over, one that several go on from is forked, and no page moves for one that a single other takes over."""
+        if len(parents) != len(names) or len(set(names)) != len(names):
+            raise ValueError(f"{len(names)} requests, of unlike names, and a parent for each, got {len(parents)}")
+        if any(not 0 <= int(p) < len(names) for p in parents):
+            raise ValueError(f"parents are 0 to {len(names) - 1}, got {list(parents)}")
+        for name in names:
+            if not self.cache.has(name):
+                raise ValueError(f"request {name!r} is not live")
+        self.raise_if_lost()
+        children: Dict[int, List[int]] = {}
+        for i, p in enumerate(parents):
+            children.setdefault(int(p), []).append(i)
+        short = {g: sum(len(c) - 1 for p, c in children.items() if self.cache.num_tokens(names[p]) % self.cache.page_size)
+                 for g in self.cache.groups}
+        over = {name for i, name in enumerate(names) if i not in children}
+        for g, n in short.items():
+            freed = len({p for r in over for p in self.cache.requests[r].tables[g]
+                         if p >= 0 and over.issuperset(self.cache.groups[g].pool.holders_of(p))})
+            if n > self.cache.groups[g].pool.num_free + freed:
+                raise OutOfPages(f"group {g}: {n} pages wanted, {self.cache.groups[g].pool.num_free} free")
+        for name in over:
+            self.cache.free_request(name)
+        for p, wanted in children.items():
+            for i in wanted[1:]:
+                self.cache.fork(names[p], ("reordered", i))
+            self.cache.rename(names[p], ("reordered", wanted[0]))
+        for i, name in enumerate(names):
+            self.cache.rename(("reordered", i), name)
+
+    def resize_cache(self, num_pages) -> None:
+        """Pools of another number of pages, with what live requests hold carried over (`CacheManager.resize`). Recorded steps hold the
+        addresses of the old ones and are forgotten; memory that is no longer needed goes back to the device."""
+        self.raise_if_lost()
+        if self.model.device.type == "cuda":
+            torch.cuda.synchronize(self.model.device)
+        self._recorded.clear()
+        self._last_ctx = None
+        self.cache.resize(num_pages)
+        if self.model.device.type == "cuda":
+            torch.cuda.synchronize(self.model.device)
+            torch.cuda.empty_cache()
 
     def finish(self, req: Hashable) -> None:
         """The request is over: its pages and its slot go back."""

@@ -53,6 +53,17 @@ class Request:
     preemptions: int = 0
     arrival: int = 0
     taken_in: float = 0.0           # when the scheduler took it in (time.monotonic), for `max_time`
+    # The request whose pages this one takes its first `shared` tokens from, where it still can when it is admitted: all that both had
+    # when this one was made but the newest, which it brings itself, to choose a token of its own from. The leader's portion ends there
+    # too, for those waiting for it.
+    leader: Optional["Request"] = None
+    shared: int = 0
+    followers: List["Request"] = field(default_factory=list)      # that wait for this one
+    mask: Optional[object] = None   # the tokens that may be chosen next (`pack_mask`); None: all
+    history_of: Optional[tuple] = None      # the (slot, preemptions) under which the device keeps its history
+    # of every token of the output, where the request asks for them
+    logprobs: List[float] = field(default_factory=list)
+    top_logprobs: List[list] = field(default_factory=list)
 
     @property
     def tokens(self) -> List[int]:
@@ -70,6 +81,10 @@ class Request:
         if start + count <= n:
             return self.prompt[start:start + count]
         return self.prompt[start:] + self.output[:start + count - n]
+
+    @property
+    def cumulative_logprob(self) -> float:
+        return float(sum(self.logprobs))
 
     @property
     def decoding(self) -> bool:
@@ -116,7 +131,7 @@ class Scheduler:
         if not request.prompt:
             raise ValueError(f"request {request.req_id!r} has an empty prompt")
         # the last generated token is never fed back, so it needs no position
-        need = len(request.prompt) + request.params.max_new_tokens - 1
+        need = len(request.prompt) + max(request.params.max_new_tokens, len(request.output)) - 1
         if need > self.max_model_len:
             raise ValueError(f"request {request.req_id!r} needs {need} positions "
                              f"({len(request.prompt)} prompt + {request.params.max_new_tokens} new); "
@@ -124,6 +139,9 @@ class Scheduler:
         request.arrival = self._arrivals
         request.taken_in = time.monotonic()
         self._arrivals += 1
+        if request.leader is not None:
+            request.shared = request.num_tokens - 1
+            request.leader.followers.append(request)
         self.waiting.append(request)
 
     @property
@@ -137,6 +155,38 @@ class Scheduler:
         self.finished.clear()
         self.num_preemptions = 0
         self._short = False
+
+    # ---------------------------------------------------------------- requests that go on from others
+
+    def _portion(self, req: Request, budget: int) -> int:
+        """Tokens of `req` that the next step takes: what is left, of the portion limit and of the budget, and no further than where
+        those that wait for it go on by themselves (at any later place a state of fixed size is no longer theirs)."""
+        end = req.num_tokens
+        for f in req.followers:
+            if req.num_computed < f.shared < end:
+                end = f.shared
+        return min(end - req.num_computed, self.max_portion, budget)
+
+    def _awaits_leader(self, req: Request) -> bool:
+        return req.leader is not None and req.leader in self.running and req.leader.num_computed < req.shared
+
+    def _take_over(self, req: Request) -> bool:
+        """Fork `req` from its leader, if that still holds what it needs and there is a page for it."""
+        if req.leader not in self.running or req.shared < 1 or not self.cache.can_fork(req.leader.req_id, req.shared):
+            return False
+        try:
+            self.cache.fork(req.leader.req_id, req.req_id, req.shared)
+        except OutOfPages:
+            return False
+        req.num_computed = req.shared
+        return True
+
+    def _leave_leader(self, req: Request) -> None:
+        """It waits for its leader no longer (which may serve it again if it is put back)."""
+        if req.leader is not None and req in req.leader.followers:
+            req.leader.followers.remove(req)
+        if req.leader is not None and req.leader.finished:
+            req.leader = None
 
     # ---------------------------------------------------------------- one step's plan
 
@@ -212,28 +262,35 @@ class Scheduler:
                 continue
             if id(req) in planned_ids:
                 continue
-            count = min(req.num_tokens - req.num_computed, self.max_portion, budget)
+            count = self._portion(req, budget)
             before = self.num_preemptions
             if self._reserve(req, req.num_computed + count, planned):
                 planned.append(ScheduledRun(req, req.num_computed, count))
                 budget -= count
             blocked |= self.num_preemptions != before
         # 3. admissions, in arrival order, while everything they need is there
-        while self.waiting and not blocked and budget > 0 and len(self.running) < self.max_num_seqs:
-            req = self.waiting[0]
-            count = min(req.num_tokens - req.num_computed, self.max_portion, budget)
+        at = 0
+        while at < len(self.waiting) and not blocked and budget > 0 and len(self.running) < self.max_num_seqs:
+            req = self.waiting[at]
+            if self._awaits_leader(req):
+                at += 1                      # (others need not wait with it)
+                continue
             if self.cache.slots.num_free == 0:
                 break
-            self.cache.add_request(req.req_id)
+            if not self._take_over(req):
+                self.cache.add_request(req.req_id)
+            count = self._portion(req, budget)
             if not self.cache.can_grow(req.req_id, req.num_computed + count):
                 self.cache.free_request(req.req_id)
+                wanted, req.num_computed = req.num_computed + count, 0
                 if not self.running:
                     raise OutOfPages(f"request {req.req_id!r} alone does not fit the page pool "
-                                     f"({req.num_computed + count} tokens wanted)")
+                                     f"({wanted} tokens wanted)")
                 self._short = True
                 break
             self.cache.grow(req.req_id, req.num_computed + count)
-            self.waiting.popleft()
+            del self.waiting[at]
+            self._leave_leader(req)
             self.running.append(req)
             planned.append(ScheduledRun(req, req.num_computed, count))
             budget -= count
@@ -258,6 +315,8 @@ class Scheduler:
             self.waiting.remove(req)
         if self.cache.has(req.req_id):
             self.cache.free_request(req.req_id)
+        self._leave_leader(req)
+        req.leader = None
         self._short = False
         self.finished.append(req)
         ended.append(req)

@@ -15,7 +15,7 @@ from . import LostStep, build
 from .attention_plan import QUERY_TILE
 from .memory_plan import MEMORY_CHUNK
 from .row_set import RowSet
-from .steering import LogitRules, TokenHistory, mask_words
+from .steering import LogitRules, TokenHistory
 from .. import debug
 
 _F32, _BF16 = 0, 1
@@ -233,7 +233,7 @@ _SIGNATURES = {
         "tnx_decode_layers": [_c_void_p, _c_int, _c_void_p],
     },
     "rows": {
-        "tnx_copy_rows": [_c_void_p, _c_int, _c_void_p, _c_int, _c_void_p, _c_ll, _c_void_p],
+        "tnx_copy_rows": [_c_void_p, _c_int, _c_void_p, _c_int, _c_void_p, _c_int, _c_ll, _c_void_p],
     },
     "steering": {
         "tnx_start_history": [_c_void_p, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_void_p],
@@ -2921,11 +2921,19 @@ class HipOps:
         if not pairs or units == 0:
             return
         self._on_this_device(rows.device, "rows")
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("copy_rows takes lists from the host and cannot be recorded into a graph")
         groups, into = rows.groups(pairs)
-        dev = self._from_host(np.array([w for g in groups for w in g] + into, dtype=np.int32), "copy_rows")
-        self._call("rows", "tnx_copy_rows", _ptr(rows.table), len(rows.tensors), _ptr(dev), len(groups),
-                   dev.data_ptr() + 16 * len(groups), units, _stream(),
-                   work=lambda: (f"{len(groups)} to {len(pairs)} rows", (len(groups) + len(pairs)) * rows.row_bytes, 0))
+        words = [w for g in groups for w in g] + into
+        host = dev = None
+        if len(words) <= self.ROW_WORDS:              # a short list goes along with the launch
+            host = (ctypes.c_int * len(words))(*words)
+        else:
+            dev = self.send_ints(np.array(words, dtype=np.int32))
+        self._call("rows", "tnx_copy_rows", rows.table.data_ptr(), len(rows.tensors), host, len(words), _ptr(dev), len(groups), units,
+                   _stream(), work=lambda: (f"{len(groups)} to {len(pairs)} rows", (len(groups) + len(pairs)) * rows.row_bytes, 0))
+
+    ROW_WORDS = 256        # of a list of rows that goes along with a launch: 4 a source with its tokens, 1 a target
 
     def token_history(self, slots: int, capacity: int) -> TokenHistory:
         """Empty histories for `slots` sequences of at most `capacity` distinct tokens."""
@@ -2977,7 +2985,7 @@ class HipOps:
             rows = given[0]
         rules = LogitRules(int(vocab), rows, slots, repetition, presence, frequency, biases, mask_rows)
         if rules.flat.size:
-            rules.device_words = self._from_host(rules.flat, "logit_rules")
+            rules.placed(self._from_host(rules.flat, "logit_rules"))
         return rules
 
     def adjust_logits(self, logits, rules: LogitRules, history: Optional[TokenHistory] = None, last=None, masks=None):
@@ -2989,36 +2997,32 @@ class HipOps:
         _want(logits, "logits", torch.float32, (rules.rows, rules.vocab))
         if rules.rows == 0:
             return logits
-        if rules.device_words is None:
-            raise ValueError("these rules were not made by logit_rules")
-        self._on_this_device(logits.device, "logits")
-        if rules.device_words.device != logits.device:
-            raise ValueError("logits and rules lie on different devices")
+        device = logits.device
+        self._on_this_device(device, "logits")
+        if rules.device_words is None or rules.device_words.device != device:
+            raise ValueError("these rules were not made by logit_rules, or lie on another device than the logits")
+        entries = used = last_at = masks_at = None
+        capacity = 0
         if rules.most_slot >= 0:
             if history is None or last is None:
                 raise ValueError("rows with a slot need the history, and the tokens chosen last")
-            _want(history.entries, "history", torch.int32)
             _want(last, "last", torch.int32)
-            if history.entries.device != logits.device or last.device != logits.device:
+            if history.entries.device != device or last.device != device:
                 raise ValueError("logits, history and last lie on different devices")
             if rules.most_slot >= min(history.slots, last.numel()):
                 raise ValueError(f"slot {rules.most_slot} is outside the history's {history.slots} or the {last.numel()} of last")
-        else:
-            history = last = None
+            entries, used, last_at, capacity = history.entries.data_ptr(), history.used.data_ptr(), last.data_ptr(), history.capacity
         if rules.most_mask >= 0:
             if masks is None:
                 raise ValueError("rows with a mask need the masks")
             _want(masks, "masks", torch.int32)
-            if masks.dim() != 2 or masks.shape[1] != mask_words(rules.vocab) or masks.device != logits.device:
-                raise ValueError(f"masks are [masks, {mask_words(rules.vocab)}] beside the logits, got {tuple(masks.shape)} on {masks.device}")
+            if masks.dim() != 2 or masks.shape[1] != rules.mask_words or masks.device != device:
+                raise ValueError(f"masks are [masks, {rules.mask_words}] beside the logits, got {tuple(masks.shape)} on {masks.device}")
             if rules.most_mask >= masks.shape[0]:
                 raise ValueError(f"mask {rules.most_mask} is outside the {masks.shape[0]} there are")
-        else:
-            masks = None
-        heads, tokens, values = rules.pieces(rules.device_words)
-        self._call("steering", "tnx_adjust_logits", _ptr(logits), _ptr(heads), _ptr(tokens), _ptr(values),
-                   _ptr(history.entries) if history else None, _ptr(history.used) if history else None,
-                   history.capacity if history else 0, _ptr(last), _ptr(masks), rules.rows, rules.vocab, _stream())
+            masks_at = masks.data_ptr()
+        self._call("steering", "tnx_adjust_logits", logits.data_ptr(), *rules.addresses, entries, used, capacity, last_at, masks_at,
+                   rules.rows, rules.vocab, _stream())
         return logits
 
     MOST_TOP = 32         # alternatives that `log_probs` gives at most
@@ -3038,12 +3042,27 @@ class HipOps:
         self._on_this_device(logits.device, "logits")
         if tokens.device != logits.device:
             raise ValueError("logits and tokens lie on different devices")
-        out = torch.empty(rows, dtype=torch.float32, device=logits.device)
-        ids = torch.empty(rows, top, dtype=torch.int32, device=logits.device) if top else None
-        best = torch.empty(rows, top, dtype=torch.float32, device=logits.device) if top else None
+        out = logits.new_empty(rows)
+        ids = tokens.new_empty(rows, top) if top else None
+        best = logits.new_empty(rows, top) if top else None
         self._call("steering", "tnx_log_probs", _ptr(logits), _ptr(tokens), _ptr(out), _ptr(ids), _ptr(best), top, rows, vocab, _stream(),
                    work=lambda: (f"{rows}x{vocab} top {top}", rows * (4 * vocab + 8 + 8 * top), 4.0 * rows * vocab))
         return out, ids, best
+
+    def send_log_probs(self, out, ids, best):
+        """What `log_probs` gave, on its way to the host; `receive_log_probs` turns it into lists once it is there."""
+        landing = [None if t is None else torch.empty(t.shape, dtype=t.dtype, pin_memory=True) for t in (out, ids, best)]
+        for host, t in zip(landing, (out, ids, best)):
+            if t is not None:
+                host.copy_(t, non_blocking=True)
+        landed = torch.cuda.Event()
+        landed.record()
+        return landing, landed
+
+    def receive_log_probs(self, sent):
+        landing, landed = sent
+        landed.synchronize()
+        return tuple(None if t is None else t.tolist() for t in landing)
 
     def synchronize(self):
         torch.cuda.synchronize(self.device)

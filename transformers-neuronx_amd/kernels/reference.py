@@ -1071,6 +1071,12 @@ class ReferenceOps:
         ids = torch.sort(x, dim=1, descending=True, stable=True).indices[:, :top]
         return out, ids.to(torch.int32), lp.gather(1, ids)
 
+    def send_log_probs(self, out, ids, best):
+        return out, ids, best
+
+    def receive_log_probs(self, sent):
+        return tuple(None if t is None else t.tolist() for t in sent)
+
     def synchronize(self):
         if self.device.type == "cuda":
             torch.cuda.synchronize(self.device)

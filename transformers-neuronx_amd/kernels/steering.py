@@ -107,7 +107,14 @@ class LogitRules:
         flat[n:n + self.num_biases] = ids
         flat[n + self.num_biases:] = add.astype(np.float32).view(np.int32)
         self.flat = flat
+        self.mask_words = mask_words(vocab)
         self.device_words: Optional[torch.Tensor] = None      # put there by the backend
+        self.addresses = (None, None, None)                   # of the rules, the biases' tokens and their values there
+
+    def placed(self, words: torch.Tensor) -> None:
+        self.device_words = words
+        at = words.data_ptr()
+        self.addresses = (at, at + 4 * self.rows * self.WORDS, at + 4 * (self.rows * self.WORDS + self.num_biases))
 
     def pieces(self, words):
         """(rules, bias tokens, bias values) of the words, in whatever memory they lie."""

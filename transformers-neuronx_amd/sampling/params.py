@@ -1,7 +1,9 @@
 """What a request asks of the sampler."""
 import operator
 from dataclasses import dataclass
-from typing import Optional, Sequence, Tuple, Union
+from typing import Callable, Dict, List, Optional, Sequence, Tuple, Union
+
+import numpy as np
 
 
 @dataclass
@@ -28,6 +30,18 @@ class SamplingParams:
     no_repeat_ngram_size  n: no run of n tokens appears twice in the prompt and what follows it; a token
                  that would complete a run seen before gets the logit -inf before anything else is done
                  (sampling.py:267-309, :334-335); 0 switches it off
+    repetition_penalty  the logit of every token of the prompt and of what follows it is divided by this if it is
+                 above zero, multiplied by it otherwise; 1.0 switches it off
+    frequency_penalty  subtracted from a token's logit for every time it was generated (the prompt does not count)
+    presence_penalty   subtracted from the logit of every token that was generated
+    logit_bias   {token: what is added to its logit}, after the penalties; -inf bars the token
+    allowed_tokens  the tokens that may be chosen: their ids, or a truth value for every token of the vocabulary; all
+                 others are barred, whatever their biases. A function of the list of tokens generated so far that gives
+                 either steers the request through a grammar; the request ends, with the reason "grammar", where
+                 nothing is allowed after a token (a request for which nothing is allowed to begin with is refused)
+    logprobs     an integer: each token is reported with its log-probability and with those of this many tokens of the
+                 largest logits (0: its own alone). They are those of the logits that the token was chosen from, with
+                 penalties, biases and bars, before temperature, top-k and top-p; None: not reported
     max_time     seconds: the request ends after the first token that arrives later than this after it was
                  taken in (stopping_criteria.py:15-35, `MaxTimeCriteria`)
     max_new_tokens  the most tokens to generate
@@ -45,8 +59,28 @@ class SamplingParams:
     ignore_eos: bool = False
     no_repeat_ngram_size: int = 0
     max_time: Optional[float] = None
+    repetition_penalty: float = 1.0
+    frequency_penalty: float = 0.0
+    presence_penalty: float = 0.0
+    logit_bias: Optional[Dict[int, float]] = None
+    allowed_tokens: Optional[Union[Sequence[int], Callable[[List[int]], Sequence[int]]]] = None
+    logprobs: Optional[int] = None
+
+    MOST_LOGPROBS = 32
 
     def __post_init__(self):
+        least, most = float(np.finfo(np.float32).tiny), float(np.finfo(np.float32).max)
+        if not least <= float(self.repetition_penalty) <= most:
+            raise ValueError(f"repetition_penalty has to be a positive number, but is {self.repetition_penalty}")
+        for name in ("frequency_penalty", "presence_penalty"):
+            if not abs(float(getattr(self, name))) <= most:
+                raise ValueError(f"{name} has to be a finite number, but is {getattr(self, name)}")
+        biases = {operator.index(t): float(b) for t, b in dict(self.logit_bias or {}).items()}
+        if any(not (abs(b) <= most or b == float("-inf")) for b in biases.values()):
+            raise ValueError("a logit bias is a finite number, or -inf for a token that must not be chosen")
+        self.biases: Tuple[Tuple[int, float], ...] = tuple(sorted(biases.items()))     # what is gone by from here on
+        if self.logprobs is not None and not (isinstance(self.logprobs, int) and 0 <= self.logprobs <= self.MOST_LOGPROBS):
+            raise ValueError(f"logprobs has to be an integer from 0 to {self.MOST_LOGPROBS}, but is {self.logprobs}")
         if self.max_new_tokens < 0:
             raise ValueError("max_new_tokens must not be negative")
         if not isinstance(self.top_k, int) or self.top_k < 0:
@@ -79,6 +113,16 @@ class SamplingParams:
         if isinstance(self.eos_token_id, int):
             return (self.eos_token_id,)
         return tuple(int(t) for t in self.eos_token_id)
+
+    @property
+    def penalised(self) -> bool:
+        """Whether the choice goes by what the request holds already."""
+        return self.repetition_penalty != 1.0 or self.frequency_penalty != 0.0 or self.presence_penalty != 0.0
+
+    @property
+    def follows_grammar(self) -> bool:
+        """Whether what is allowed is asked anew for every token."""
+        return callable(self.allowed_tokens)
 
     @property
     def greedy(self) -> bool:
