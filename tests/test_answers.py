@@ -1,0 +1,571 @@
+"""Several answers to one prompt, steered and scored, through the engine: on the host with the plain renditions of the kernels, and on the
+GPU with the kernels. Forked and resized caches are compared with requests that were computed by themselves."""
+import dataclasses
+import random
+
+import numpy as np
+import pytest
+import torch
+
+import gubulorn_cases
+import sunatar_cases
+import tadolix_cases
+import zudusun_cases
+from transformers_neuronx_amd.cache import CacheManager, OutOfPages, OutOfSlots, PagePool
+from transformers_neuronx_amd.config import EngineConfig
+from transformers_neuronx_amd.engine import StepEntry
+from transformers_neuronx_amd.engine.engine import LLMEngine
+from transformers_neuronx_amd.engine.factory import runner_from_folder
+from transformers_neuronx_amd.kernels import make_ops
+from transformers_neuronx_amd.parts.base import CacheNeed
+from transformers_neuronx_amd.sampling import Sampler, SamplingParams, Steering
+
+BOTH = pytest.mark.parametrize("kernels", ["reference", pytest.param("hip", marks=pytest.mark.gpu)])
+
+
+def device_of(kernels):
+    return "cuda:0" if kernels == "hip" else "cpu"
+
+
+def engine_of(folder, kernels, max_tokens=640, max_num_seqs=8, **kw):
+    cfg = EngineConfig(dtype="float32", kernels=kernels, device=device_of(kernels), page_size=16, max_tokens=max_tokens,
+                       max_num_seqs=max_num_seqs, **kw)
+    return LLMEngine(runner_from_folder(folder, cfg), cfg)
+
+
+def prompts_of(vocab, lengths, seed):
+    rng = random.Random(seed)
+    return [[rng.randrange(3, vocab) for _ in range(n)] for n in lengths]
+
+
+# ---------------------------------------------------------------- pools and tables
+
+def test_shared_pages_are_free_when_the_last_holder_gives_them_back():
+    pool = PagePool(4)
+    a = pool.allocate(2, "a")
+    pool.share(a, "b")
+    assert pool.holders_of(a[0]) == ("a", "b") and pool.num_free == 2
+    with pytest.raises(ValueError, match="already"):
+        pool.share(a[:1], "b")
+    with pytest.raises(ValueError, match="nobody"):
+        pool.share([p for p in range(4) if p not in a][:1], "c")
+    pool.free(a, "a")
+    assert pool.num_free == 2 and pool.holder_of(a[0]) == "b"
+    with pytest.raises(ValueError, match="held by"):
+        pool.free(a, "a")
+    with pytest.raises(ValueError, match="twice"):
+        pool.free([a[0], a[0]], "b")
+    pool.rename(a, "b", "c")
+    pool.free(a, "c")
+    assert pool.num_free == 4
+    pool.check()
+
+
+def test_where_pages_go_when_a_pool_is_packed():
+    pool = PagePool(6)
+    held = pool.allocate(6, "a")
+    pool.free([p for p in held if p in (0, 3, 4)], "a")
+    where = pool.packed(6)
+    assert where == {1: 1, 2: 2, 5: 0}
+    with pytest.raises(OutOfPages):
+        pool.packed(2)
+    pool.repack(where, 3)
+    assert pool.num_free == 0 and pool.num_pages == 3 and pool.holder_of(0) == "a"
+    pool.check()
+
+
+def manager(kernels="reference", window=40, state=False, num_pages=40, max_seqs=8, dtype=torch.float32):
+    needs = {0: CacheNeed("paged", kv_heads=2, head_size=16), 1: CacheNeed("paged", kv_heads=1, head_size=8)}
+    if window:
+        needs[2] = CacheNeed("paged", kv_heads=1, head_size=16, window=window)
+    if state:
+        needs[3] = CacheNeed("state", state_shapes=(("m", (3, 5)), ("n", (7,))))
+    dev = device_of(kernels)
+    return CacheManager(needs, 16, num_pages, max_seqs, dtype, dev, page_pad_bytes=32, ops=make_ops(kernels, dtype, dev))
+
+
+def fill(m, req, start, values):
+    """The keys and values of tokens from `start` on, as numbers that name them."""
+    r = m.requests[req]
+    for cid, lc in m.caches.items():
+        if lc.group is None:
+            continue
+        for i, v in enumerate(values):
+            page = r.tables[lc.group][(start + i) // 16]
+            lc.pages["k"][page, :, (start + i) % 16] = v + cid
+            lc.pages["v"][page, :, :, (start + i) % 16] = -v - cid
+
+
+def holds(m, req, values):
+    r = m.requests[req]
+    assert r.num_tokens == len(values)
+    for cid, lc in m.caches.items():
+        if lc.group is None:
+            continue
+        g = m.groups[lc.group]
+        first = 0 if g.window is None else max(0, len(values) - g.window + 1)
+        for i in range(first, len(values)):
+            page = r.tables[lc.group][i // 16]
+            assert page >= 0 and (lc.pages["k"][page, :, i % 16] == values[i] + cid).all(), (req, cid, i)
+            assert (lc.pages["v"][page, :, :, i % 16] == -values[i] - cid).all(), (req, cid, i)
+
+
+@BOTH
+@pytest.mark.parametrize("state", [False, True])
+def test_requests_forked_grown_ended_compacted_and_resized_in_any_order(kernels, state):
+    m = manager(kernels, state=state, num_pages=60)
+    rng = random.Random(5)
+    live, states, named = {}, {}, 0
+    for turn in range(120):
+        what = rng.choice(["new", "grow", "grow", "fork", "fork", "end", "compact", "resize", "rename"])
+        m.check()
+        if what == "new" and len(live) < 8:
+            name, named = f"r{named}", named + 1
+            m.add_request(name)
+            live[name], states[name] = [], 0.0
+        elif what == "grow" and live:
+            name = rng.choice(sorted(live))
+            n = rng.choice([1, 1, 5, 16, 23])
+            if m.can_grow(name, len(live[name]) + n):
+                m.grow(name, len(live[name]) + n)
+                values = [rng.randrange(1, 1 << 12) for _ in range(n)]
+                fill(m, name, len(live[name]), values)
+                m.advance(name, n)
+                live[name] = live[name] + values
+                states[name] += 1.5
+                if state:
+                    for t in m.caches[3].state.values():
+                        t[m.slot_of(name)] = states[name]
+        elif what == "fork" and live:
+            name = rng.choice(sorted(live))
+            n = len(live[name]) if state else rng.randint(0, len(live[name]))
+            child, named = f"r{named}", named + 1
+            if not m.can_fork(name, n):
+                with pytest.raises(ValueError):
+                    m.fork(name, child, n)
+            else:
+                try:
+                    m.fork(name, child, n)
+                    live[child], states[child] = live[name][:n], states[name]
+                except (OutOfPages, OutOfSlots):
+                    assert not m.has(child)
+        elif what == "end" and len(live) > 2:
+            name = rng.choice(sorted(live))
+            m.free_request(name)
+            del live[name], states[name]
+        elif what == "compact":
+            m.compact()
+            for g in m.groups.values():
+                held = g.pool.num_pages - g.pool.num_free
+                assert all(g.pool.holders_of(p) for p in range(held))
+            assert m.compact() == 0
+        elif what == "resize":
+            size = rng.randint(30, 70)
+            if all(g.pool.num_pages - g.pool.num_free <= size for g in m.groups.values()):
+                m.resize(size)
+                assert all(g.pool.num_pages == size and len(m.caches[g.cache_ids[0]].pages["k"]) == size for g in m.groups.values())
+            else:
+                with pytest.raises(OutOfPages):
+                    m.resize(size)
+        elif what == "rename" and live:
+            name = rng.choice(sorted(live))
+            m.rename(name, name + "x")
+            live[name + "x"], states[name + "x"] = live.pop(name), states.pop(name)
+        for name in live:
+            holds(m, name, live[name])
+            if state and live[name]:
+                assert all((t[m.slot_of(name)] == states[name]).all() for t in m.caches[3].state.values())
+    assert named > 20
+    m.reset()
+    m.check()
+
+
+def test_forks_that_are_refused():
+    m = manager(num_pages=3, window=20, max_seqs=2)
+    m.add_request("a")
+    m.grow("a", 40)
+    m.advance("a", 40)                      # the window's first page is gone: blocks 0 of positions up to 20
+    assert m.can_fork("a", 40) and not m.can_fork("a", 30) and not m.can_fork("a", 41) and not m.can_fork("a", -1)
+    assert not m.can_fork("b", 0)
+    with pytest.raises(ValueError, match="already live"):
+        m.fork("a", "a")
+    with pytest.raises(OutOfPages):
+        m.fork("a", "b")                    # no page for the one that is not full
+    assert not m.has("b") and m.slots.num_free == 1
+    m.check()
+    m.add_request("c")
+    m.free_request("a")
+    m.grow("c", 16)
+    m.advance("c", 16)
+    m.add_request("d")
+    with pytest.raises(OutOfSlots):
+        m.fork("c", "e")
+    m.check()
+    no_kernels = CacheManager({0: CacheNeed("paged", kv_heads=1, head_size=8)}, 16, 4, 2, torch.float32, "cpu")
+    no_kernels.add_request("a")
+    no_kernels.grow("a", 3)
+    no_kernels.advance("a", 3)
+    with pytest.raises(RuntimeError, match="backend"):
+        no_kernels.fork("a", "b")
+    no_kernels.check()
+    with pytest.raises(ValueError):
+        m.resize(0)
+
+
+# ---------------------------------------------------------------- answers that share a prompt
+
+@BOTH
+@pytest.mark.parametrize("run_ahead", [True, False])
+@pytest.mark.parametrize("seqs, tokens, chunk", [(8, 640, None), (8, 640, 11), (3, 640, None), (8, 256, 9)])
+def test_samples_are_what_requests_of_their_own_give(tiny_folders, kernels, run_ahead, seqs, tokens, chunk):
+    """Also where slots or pages run out, so that some of them are computed by themselves, put back and admitted again."""
+    folder, cfg, _ = tiny_folders["A"]
+    prompts = prompts_of(cfg["vocab_size"], [37, 16, 1, 2, 33], 3)
+    params = SamplingParams(max_new_tokens=14, temperature=1.3, top_k=40, seed=11, ignore_eos=True)
+    alone = engine_of(folder, kernels, run_ahead=run_ahead)
+    want = [alone.generate([p], dataclasses.replace(params, seed=11 + i))[0] for p in prompts for i in range(4)]
+    engine = engine_of(folder, kernels, tokens, seqs, chunk_size=chunk, run_ahead=run_ahead)
+    assert engine.generate(prompts, params, samples=4) == want
+    engine.runner.cache.check()
+    assert not engine.runner.cache.requests and all(g.pool.num_free == g.pool.num_pages for g in engine.runner.cache.groups.values())
+
+
+@BOTH
+def test_a_prompt_is_computed_once(tiny_folders, kernels):
+    folder, cfg, _ = tiny_folders["A"]
+    engine = engine_of(folder, kernels)
+    names = engine.add_samples(prompts_of(cfg["vocab_size"], [50], 1)[0], SamplingParams(max_new_tokens=4, seed=1), 5, "p")
+    assert names == ["p", ("p", 1), ("p", 2), ("p", 3), ("p", 4)]
+    seen = []
+    step = engine.runner.step
+    engine.runner.step = lambda entries, **kw: (seen.append([len(e.tokens) for e in entries]), step(entries, **kw))[1]
+    engine.step()
+    engine.step()
+    cache = engine.runner.cache
+    assert seen == [[49], [1] * 5]
+    full = [cache.requests[n].tables["full"][:3] for n in names]
+    assert all(t == full[0] for t in full) and len({cache.requests[n].tables["full"][3] for n in names}) == 5
+    cache.check()
+    engine.abort_request("p")
+    cache.check()
+    engine.run()
+    assert [len(engine.requests[n].output) for n in names[1:]] == [4] * 4
+
+
+CASES = {"sunatar": (sunatar_cases, "a"), "gubulorn": (gubulorn_cases, "a"), "tadolix": (tadolix_cases, "a"), "zudusun": (zudusun_cases, "a")}
+
+
+@BOTH
+@pytest.mark.parametrize("design", list(CASES))
+def test_samples_of_designs_that_keep_state(design, kernels):
+    module, name = CASES[design]
+    cfg = module.config(name)
+    w = module.weights(cfg, 4)
+    prompt = module.requests(cfg, [41], 2)["r0"]
+    params = SamplingParams(max_new_tokens=7, temperature=1.1, seed=5, ignore_eos=True)
+
+    def fresh():
+        runner = module.runner(cfg, w, kernels=kernels, device=device_of(kernels), max_tokens=512, max_seqs=5)
+        ecfg = EngineConfig(dtype="float32", page_size=16, max_tokens=512, max_num_seqs=5, device=device_of(kernels), kernels=kernels)
+        return LLMEngine(runner, ecfg)
+    want = [fresh().generate([prompt], dataclasses.replace(params, seed=5 + i))[0] for i in range(4)]
+    engine = fresh()
+    forks = []
+    fork = engine.runner.cache.fork
+    engine.runner.cache.fork = lambda *a: (forks.append(a), fork(*a))[1]
+    assert engine.generate([prompt], params, samples=4) == want
+    assert len(forks) == 3
+    engine.runner.cache.check()
+
+
+@BOTH
+def test_a_request_forked_midway(tiny_folders, kernels):
+    folder, cfg, _ = tiny_folders["B"]
+    prompt = prompts_of(cfg["vocab_size"], [21], 8)[0]
+    params = SamplingParams(max_new_tokens=20, temperature=1.2, seed=3, ignore_eos=True, logprobs=1)
+    engine = engine_of(folder, kernels)
+    engine.add_request(prompt, params, "a")
+    for _ in range(6):
+        engine.step()
+    have = [t for t in engine.requests["a"].output if t >= 0]
+    assert 3 <= len(have) < 20
+    greedy = dataclasses.replace(params, do_sample=False)
+    assert engine.fork_request("a", greedy, "b") == "b"
+    again = engine.fork_request("a")
+    engine.run()
+    a, b, c = (engine.requests[n] for n in ("a", "b", again))
+    alone = engine_of(folder, kernels)
+    assert a.output == alone.generate([prompt], params)[0]
+    assert b.output[:len(have)] == have and b.output[len(have):] == alone.generate(
+        [prompt + have], dataclasses.replace(greedy, max_new_tokens=20 - len(have)))[0]
+    assert c.output[:len(have)] == have and len(c.output) == 20 and len(c.logprobs) == len(c.top_logprobs) == 20
+    with pytest.raises(ValueError, match="tokens already"):
+        engine.fork_request("a")
+    engine.runner.cache.check()
+
+
+@BOTH
+def test_the_cache_resized_between_steps(tiny_folders, kernels):
+    folder, cfg, _ = tiny_folders["A"]
+    prompts = prompts_of(cfg["vocab_size"], [30, 45, 5], 6)
+    params = SamplingParams(max_new_tokens=24, do_sample=False, ignore_eos=True)
+    want = engine_of(folder, kernels).generate(prompts, params)
+    engine = engine_of(folder, kernels)
+    names = [engine.add_request(p, params) for p in prompts]
+    for n, size in enumerate([40, 13, 13, 80, 15, 14]):
+        engine.step()
+        engine.step()
+        engine.resize_cache(size)
+        engine.runner.cache.check()
+    with pytest.raises(OutOfPages):
+        engine.resize_cache(3)
+    engine.run()
+    assert [engine.requests[n].output for n in names] == want
+
+
+# ---------------------------------------------------------------- steered and scored
+
+def adjusted_row(row, request, index, vocab):
+    """The logits that token `index` of the request was chosen from, in 64 bits."""
+    p, x = request.params, row.double().numpy().copy()
+    before = request.output[:index]
+    for t in set(request.prompt) | set(before):
+        times = before.count(t)
+        x[t] = x[t] / p.repetition_penalty if x[t] > 0 else x[t] * p.repetition_penalty
+        x[t] -= p.frequency_penalty * times + (p.presence_penalty if times else 0.0)
+    for t, b in (p.logit_bias or {}).items():
+        x[t] = -np.inf if b == -np.inf else x[t] + b
+    if p.allowed_tokens is not None:
+        allowed = p.allowed_tokens(list(before)) if callable(p.allowed_tokens) else p.allowed_tokens
+        keep = np.zeros(vocab, dtype=bool)
+        keep[np.asarray(allowed)] = True
+        x[~keep] = -np.inf
+    return x
+
+
+def check_steered(engine, vocab, run):
+    """Every chosen token is the largest of the steered logits, and what is said of it is their log-probability."""
+    rows = []
+
+    def keep(requests, logits):
+        rows.extend((q, len(q.output), x.clone()) for q, x in zip(requests, logits.cpu()))
+    engine.logits_hook = keep
+    run()
+    seen = 0
+    for q, index, row in rows:
+        if index >= len(q.output):
+            continue                                  # a step started when the request had ended
+        x = adjusted_row(row, q, index, vocab)
+        scale = np.abs(x[np.isfinite(x)]).max()
+        # two roundings a penalty and bias, of values up to the scale: the largest is met to 1e-6 of it
+        assert x[q.output[index]] >= x.max() - 1e-6 * scale, (q.req_id, index)
+        if q.params.logprobs is not None:
+            lp = x - x.max() - np.log(np.exp(x - x.max()).sum())
+            assert abs(q.logprobs[index] - lp[q.output[index]]) <= 1e-6 * (1 + scale)
+            top = q.top_logprobs[index]
+            assert len(top) == q.params.logprobs and [v for _, v in top] == sorted((v for _, v in top), reverse=True)
+            if top:
+                assert top[0][0] == q.output[index]
+                assert all(abs(v - lp[t]) <= 1e-6 * (1 + scale) or (np.isneginf(v) and np.isneginf(lp[t])) for t, v in top)
+        seen += 1
+    return seen
+
+
+@BOTH
+@pytest.mark.parametrize("run_ahead", [True, False])
+@pytest.mark.parametrize("tokens", [640, 160])
+def test_steered_requests_beside_plain_ones(tiny_folders, kernels, run_ahead, tokens):
+    """With room for all, and with so little that requests are put back and their histories begun again."""
+    folder, cfg, _ = tiny_folders["A"]
+    vocab = cfg["vocab_size"]
+    rng = random.Random(4)
+    engine = engine_of(folder, kernels, tokens, run_ahead=run_ahead)
+    base = dict(max_new_tokens=25, do_sample=False, ignore_eos=True)
+    sets = [dict(), dict(repetition_penalty=1.6), dict(presence_penalty=0.8, frequency_penalty=0.5, logprobs=3), dict(logprobs=0),
+            dict(logit_bias={t: rng.uniform(-2, 2) for t in range(100, 140)}), dict(allowed_tokens=list(range(0, vocab, 3)), logprobs=5),
+            dict(repetition_penalty=0.7, frequency_penalty=-0.2, logit_bias={7: float("-inf"), 8: 1.0}, allowed_tokens=np.arange(vocab) % 2 == 0)]
+    for i, (s, p) in enumerate(zip(sets, prompts_of(vocab, [20, 31, 3, 17, 40, 1, 26], 9))):
+        engine.add_request(p, SamplingParams(**base, **s), i)
+    assert check_steered(engine, vocab, engine.run) == 7 * 25
+    if tokens == 160:
+        assert engine.scheduler.num_preemptions > 0
+    engine.runner.cache.check()
+
+
+@BOTH
+def test_a_grammar(tiny_folders, kernels):
+    """Tokens that have to rise by at most five each time, and end where none is left."""
+    folder, cfg, _ = tiny_folders["A"]
+    vocab = cfg["vocab_size"]
+
+    def rising(output):
+        last = output[-1] if output else vocab - 41
+        return [t for t in range(last + 1, last + 6) if t < vocab]
+    engine = engine_of(folder, kernels)
+    prompts = prompts_of(vocab, [9, 12], 2)
+    engine.add_request(prompts[0], SamplingParams(max_new_tokens=60, do_sample=False, allowed_tokens=rising, logprobs=2), "a")
+    engine.add_request(prompts[1], SamplingParams(max_new_tokens=5, do_sample=False, ignore_eos=True), "b")
+    ends = {}
+
+    def run():
+        while engine.has_work:
+            for o in engine.step():
+                if o.finished:
+                    ends[o.req_id] = o
+    assert check_steered(engine, vocab, run) == len(engine.requests["a"].output) + 5
+    out = engine.requests["a"].output
+    assert all(0 < b - a <= 5 for a, b in zip(out, out[1:])) and out[-1] == vocab - 1
+    assert ends["a"].finish_reason == "grammar" and ends["a"].token == vocab - 1 and ends["b"].finish_reason == "length"
+    assert ends["a"].logprob == engine.requests["a"].logprobs[-1] and len(ends["a"].top_logprobs) == 2
+
+
+@BOTH
+def test_the_best_of_several(tiny_folders, kernels):
+    folder, cfg, _ = tiny_folders["A"]
+    prompts = prompts_of(cfg["vocab_size"], [12, 30], 7)
+    params = SamplingParams(max_new_tokens=8, temperature=1.5, seed=2, ignore_eos=True)
+    engine = engine_of(folder, kernels)
+    every = engine.generate_requests(prompts, dataclasses.replace(params, logprobs=0), samples=5)
+    best = engine.generate(prompts, params, samples=2, best_of=5)
+    want = [q.output for family in every for q in sorted(family, key=lambda q: -q.cumulative_logprob)[:2]]
+    assert best == want
+    for bad in (dict(samples=0), dict(samples=3, best_of=2)):
+        with pytest.raises(ValueError):
+            engine.generate(prompts, params, **bad)
+
+
+def test_params_that_are_refused(tiny_folders):
+    nan, inf = float("nan"), float("inf")
+    for bad in (dict(repetition_penalty=0.0), dict(repetition_penalty=-1.0), dict(repetition_penalty=nan), dict(repetition_penalty=inf),
+                dict(repetition_penalty=1e-50), dict(frequency_penalty=nan), dict(presence_penalty=inf), dict(logit_bias={3: nan}),
+                dict(logit_bias={3: inf}), dict(logit_bias={3: 1e300}), dict(logprobs=-1), dict(logprobs=33), dict(logprobs=1.5)):
+        with pytest.raises(ValueError):
+            SamplingParams(**bad)
+    folder, cfg, _ = tiny_folders["A"]
+    engine = engine_of(folder, "reference")
+    vocab = cfg["vocab_size"]
+    for bad in (dict(logit_bias={vocab: 1.0}), dict(logit_bias={-1: 1.0}), dict(allowed_tokens=[vocab]), dict(allowed_tokens=[]),
+                dict(allowed_tokens=lambda out: []), dict(allowed_tokens=np.ones(vocab - 1, dtype=bool)),
+                dict(allowed_tokens=[5], logit_bias={5: -inf}), dict(allowed_tokens=[2], ban_eos=True, eos_token_id=2)):
+        with pytest.raises(ValueError):
+            engine.add_request([3, 4, 5], SamplingParams(**bad))
+    for count, params in ((0, SamplingParams()), (2, SamplingParams(max_new_tokens=0))):
+        with pytest.raises(ValueError):
+            engine.add_samples([3], params, count)
+    assert not engine.has_work and not engine.requests
+    engine.add_request([3], SamplingParams(), ("p", 1))
+    with pytest.raises(ValueError, match="already live"):
+        engine.add_samples([3], SamplingParams(), 2, "p")
+    with pytest.raises(KeyError):
+        engine.fork_request("nobody")
+    # a sampler that keeps no histories has nothing to penalise by
+    ops = make_ops("reference", torch.float32, "cpu")
+    with pytest.raises(ValueError, match="slot"):
+        Sampler(ops, "cpu").draw(torch.zeros(1, 4), [SamplingParams(repetition_penalty=2.0)], [0], steering=[Steering(0)])
+
+
+@BOTH
+def test_rules_follow_the_batch(kernels):
+    """Rows that change places, leave and return, with one sampler: each batch goes by its own rules and masks."""
+    dev = device_of(kernels)
+    ops = make_ops(kernels, torch.float32, dev)
+    last = torch.full((4,), -1, dtype=torch.int32, device=dev)
+    sampler = Sampler(ops, dev, slots=4, capacity=50, last=last)
+    masks = [np.array([0b1110, 0], dtype=np.int32), np.array([0b0110, 0], dtype=np.int32)]
+    greedy = dict(do_sample=False)
+    rows = [(SamplingParams(presence_penalty=5.0, **greedy), 0, None), (SamplingParams(**greedy), 1, masks[0]),
+            (SamplingParams(logit_bias={3: 9.0}, **greedy), 2, masks[1]), (SamplingParams(logit_bias={4: 2.5}, **greedy), 3, None)]
+    logits = torch.zeros(4, 50)
+    logits[:, 9], logits[:, 3], logits[:, 2] = 2.0, 1.0, 0.5
+    want = {0: [9, 3, 2], 1: [3] * 9, 2: [2] * 9, 3: [4] * 9}
+    turns = {i: 0 for i in range(4)}
+    for batch in ([0, 1, 2, 3], [3, 1], [0, 2], [2, 0], [1], [1], [2, 1]):
+        steering = [Steering(rows[i][1], start=([], []) if turns[i] == 0 else None, mask=rows[i][2]) for i in batch]
+        drawn = sampler.draw(logits[batch].to(dev), [rows[i][0] for i in batch], [0] * len(batch), steering=steering)
+        for i, t in zip(batch, drawn.tolist()):
+            assert t == want[i][turns[i]], (batch, i)
+            last[rows[i][1]] = t
+            turns[i] += 1
+
+
+# ---------------------------------------------------------------- the user's model class
+
+def model_of(folder, kernels, batch_size=4, **kw):
+    from transformers_neuronx_amd import OPTForSampling
+    return OPTForSampling.from_pretrained(folder, batch_size=batch_size, amp="f32", n_positions=64, page_size=16, kernels=kernels,
+                                          device=device_of(kernels), **kw).load()
+
+
+@BOTH
+def test_sequences_from_the_entry_point(tiny_folders, kernels):
+    folder, cfg, _ = tiny_folders["A"]
+    ids = torch.tensor(prompts_of(cfg["vocab_size"], [10, 10], 1))
+    model = model_of(folder, kernels, 6)
+    one = [model.sample(ids[b:b + 1], 18, top_k=20, seed=7 + 3 * b + i) for b in range(2) for i in range(3)]
+    out = model.sample(ids, 18, top_k=20, seed=7, num_return_sequences=3)
+    assert torch.equal(out, torch.cat(one))
+    best = model.sample(ids, 18, top_k=20, seed=7, best_of=3)
+    score = model.log_probs(out)[:, 10:].sum(1)
+    # the sums are of the same log-probabilities, but that the token no answer may have is barred in the one and not in the other
+    assert best.shape == (2, 18) and all((best[b].unsqueeze(0) == out[3 * b:3 * b + 3]).all(1).any() for b in range(2))
+    for b in range(2):
+        chosen = (best[b].unsqueeze(0) == out[3 * b:3 * b + 3]).all(1).nonzero()[0, 0]
+        assert score[3 * b + chosen] >= score[3 * b:3 * b + 3].max() - 0.05
+    greedy = model.sample(ids, 18, top_k=1, repetition_penalty=1e6)
+    assert all(len(set(row.tolist()[10:])) == 8 and not set(row.tolist()[10:]) & set(row.tolist()[:10]) for row in greedy)
+    assert (model.sample(ids, 14, top_k=5, allowed_tokens=[40, 41])[:, 10:] // 2 == 20).all()
+    for bad in (dict(num_return_sequences=0), dict(num_return_sequences=3, best_of=2)):
+        with pytest.raises(ValueError):
+            model.sample(ids, 18, **bad)
+
+
+@BOTH
+def test_a_text_scored(tiny_folders, kernels):
+    import plain_opt
+    folder, cfg, weights = tiny_folders["A"]
+    rows = prompts_of(cfg["vocab_size"], [30, 17], 5)
+    ids = torch.zeros(2, 30, dtype=torch.long)
+    ids[0], ids[1, 13:] = torch.tensor(rows[0]), torch.tensor(rows[1])
+    for portion in (2048, 7):
+        got = model_of(folder, kernels, max_num_batched_tokens=portion).log_probs(ids, start_ids=[0, 13])
+        for b, toks in enumerate(rows):
+            lp = torch.log_softmax(plain_opt.forward_logits(weights, cfg, toks).double(), -1)
+            want = lp[torch.arange(len(toks) - 1), torch.tensor(toks[1:])]
+            first = 30 - len(toks) + 1
+            assert (got[b, :first] == 0).all() and torch.allclose(got[b, first:].double(), want, atol=3e-5)
+
+
+@BOTH
+def test_rows_reordered_and_sequences_forked(tiny_folders, kernels):
+    folder, cfg, _ = tiny_folders["A"]
+    vocab = cfg["vocab_size"]
+    ids = torch.tensor(prompts_of(vocab, [19] * 4, 3))
+    model = model_of(folder, kernels)
+    model.forward(ids)
+    texts = ids.tolist()
+    nxt = 19
+    for beams in ([1, 1, 0, 1], [3, 2, 1, 0], [2, 2, 2, 2], [0, 1, 2, 3]):
+        model.reorder_cache(beams)
+        texts = [list(texts[b]) for b in beams]
+        new = torch.tensor(prompts_of(vocab, [4], nxt)[0]).unsqueeze(1)
+        texts = [t + [int(n)] for t, n in zip(texts, new)]
+        logits = model.forward(new, cache_ids=[nxt])
+        nxt += 1
+        model.engine.runner.cache.check()
+    want = model_of(folder, kernels).forward(torch.tensor(texts))
+    assert torch.allclose(logits, want, atol=2e-5 * float(want.abs().max()))
+    for bad in ([0, 1, 2], [0, 1, 2, 4], [0, 1, 2, 3, 4]):
+        with pytest.raises(ValueError):
+            model.reorder_cache(bad) if len(bad) != 3 else model.engine.runner.reorder([("row", b) for b in range(4)], bad)
+    from transformers_neuronx_amd import ContinuousBatchingConfig, NeuronConfig
+    model = model_of(folder, kernels, neuron_config=NeuronConfig(continuous_batching=ContinuousBatchingConfig(max_num_seqs=4)))
+    model.forward(ids[:1], cache_ids=torch.arange(19).unsqueeze(0), start_ids=[2])
+    model.fork_sequence(2, 0)
+    a = model.forward(torch.tensor([[5], [6]]), cache_ids=torch.tensor([[19], [19]]), start_ids=[0, 2])
+    fresh = model_of(folder, kernels)
+    want = fresh.forward(torch.cat([ids[:1].repeat(2, 1), torch.tensor([[5], [6]])], 1))
+    assert torch.allclose(a, want, atol=2e-5 * float(want.abs().max()))
+    with pytest.raises(ValueError):
+        model.fork_sequence(3, 1)
+    with pytest.raises(ValueError):
+        model.fork_sequence(0, 0)

@@ -215,13 +215,54 @@ class CausalLMForSampling:
 
     __call__ = forward
 
+    def reorder_cache(self, beam_idx) -> None:
+        """Row b goes on from what row `beam_idx[b]` holds (decoder.py:2262-2319, what a search over beams asks for after each choice):
+        rows of a parent share its full pages, and only the page that is not full, and the fixed state, are copied. The rows are those
+        of the last `forward` that began a batch."""
+        runner = self._need_engine().runner
+        parents = [int(p) for p in torch.as_tensor(beam_idx).flatten()]
+        runner.reorder([("row", b) for b in range(len(parents))], parents)
+
+    def fork_sequence(self, seq_id: int, new_seq_id: int) -> None:
+        """Sequence `new_seq_id` of the continuous-batching form goes on from what `seq_id` holds; one that it held before is over."""
+        runner = self._need_engine().runner
+        if int(seq_id) == int(new_seq_id) or not runner.cache.has(("seq", int(seq_id))):
+            raise ValueError(f"sequence {seq_id} holds nothing that sequence {new_seq_id} could go on from")
+        runner.finish(("seq", int(new_seq_id)))
+        runner.fork(("seq", int(seq_id)), ("seq", int(new_seq_id)))
+
+    @torch.no_grad()
+    def log_probs(self, input_ids, start_ids=None) -> torch.Tensor:
+        """float32 `[batch, tokens]` on the host: the log-probability of every token under those before it in its row (0 for a row's
+        first token, and for its padding): how likely the model finds a text. Rows that `forward` holds are left as they are; there
+        has to be a slot, and pages for a row, beside them."""
+        engine = self._need_engine()
+        runner = engine.runner
+        rows = self._rows(input_ids, start_ids)
+        out = torch.zeros(len(rows), torch.as_tensor(input_ids).shape[-1])
+        portion = self.engine_config.max_num_batched_tokens
+        for b, toks in enumerate(rows):
+            key = ("scored", b)
+            try:
+                for at in range(0, len(toks) - 1, portion):
+                    part = toks[at:min(at + portion, len(toks) - 1)]
+                    logits = runner.step([StepEntry(key, part, list(range(len(part))))])
+                    wanted = torch.tensor(toks[at + 1:at + 1 + len(part)], dtype=torch.int32).to(logits.device)
+                    first = out.shape[1] - len(toks) + at + 1
+                    out[b, first:first + len(part)] = runner.ops.log_probs(logits, wanted)[0].cpu()
+            finally:
+                runner.finish(key)
+        return out
+
     # ---------------------------------------------------------------- generation
 
     @torch.no_grad()
     def sample(self, input_ids, sequence_length: int, start_ids=None, top_k: int = 50, streamer=None,
                temperature: float = 1.0, top_p: float = 1.0, seed: int = 0,
                generation_config: Optional[GenerationConfig] = None,
-               no_repeat_ngram_size: Optional[int] = None, eos_token_id: Optional[int] = None) -> torch.Tensor:
+               no_repeat_ngram_size: Optional[int] = None, eos_token_id: Optional[int] = None,
+               repetition_penalty: float = 1.0, frequency_penalty: float = 0.0, presence_penalty: float = 0.0, logit_bias=None,
+               allowed_tokens=None, num_return_sequences: int = 1, best_of: Optional[int] = None) -> torch.Tensor:
         """`[batch, sequence_length]`: the prompts and what follows them, up to a total
         length of `sequence_length`. As the reference's loop (sampling.py:131-180) it
         never picks the end-of-sequence token and keeps the `top_k` largest logits;
@@ -229,7 +270,12 @@ class CausalLMForSampling:
         `generation_config`, those options decide instead (sampling.py:33-105).
         `eos_token_id`: the token the loop never picks, where it is not the configuration's.
         `no_repeat_ngram_size`: no run of that many tokens appears twice in a row's prompt and what
-        follows it (the option of the reference's other loop, sampling.py:382-394)."""
+        follows it (the option of the reference's other loop, sampling.py:382-394).
+        `repetition_penalty`, `frequency_penalty`, `presence_penalty`, `logit_bias`, `allowed_tokens`: see
+        `SamplingParams`, the same for every row. `num_return_sequences`: that many answers to each prompt, one behind
+        the other, `[batch * num_return_sequences, sequence_length]`; they share the prompt's pages where they run
+        beside one another (`batch_size` counts them). `best_of`: so many are made, and of each prompt's those with the
+        largest sum of log-probabilities kept, the largest first."""
         engine = self._need_engine()
         rows = self._rows(input_ids, start_ids)
         gen = generation_config or self.neuron_config.on_device_generation
@@ -239,6 +285,13 @@ class CausalLMForSampling:
         width = prompts.shape[1]
         if sequence_length <= width:
             return prompts[:, :sequence_length].clone()
+        made = num_return_sequences if best_of is None else best_of
+        if num_return_sequences < 1 or made < num_return_sequences:
+            raise ValueError(f"num_return_sequences ({num_return_sequences}) is at least 1 and no more than best_of ({best_of})")
+        if streamer is not None and made > num_return_sequences:
+            raise ValueError("which answers are kept is known at their end: best_of has nothing to stream")
+        steered = dict(repetition_penalty=repetition_penalty, frequency_penalty=frequency_penalty, presence_penalty=presence_penalty,
+                       logit_bias=logit_bias, allowed_tokens=allowed_tokens, logprobs=0 if made > num_return_sequences else None)
         params = []
         for b, toks in enumerate(rows):
             new = sequence_length - width
@@ -252,19 +305,21 @@ class CausalLMForSampling:
                 if gen.global_top_k is not None:
                     k = min(k, int(gen.global_top_k)) if k > 0 else int(gen.global_top_k)
                 p = SamplingParams(max_new_tokens=new, do_sample=gen.do_sample, temperature=float(line(gen.temperature)),
-                                   top_k=k, top_p=float(line(gen.top_p)), seed=seed + b,
+                                   top_k=k, top_p=float(line(gen.top_p)), seed=seed + b * made,
                                    min_tokens_to_keep=int(line(gen.top_p_min_tokens)), deterministic=gen.deterministic,
                                    eos_token_id=gen.eos_token_id, ignore_eos=gen.eos_token_id is None,
-                                   no_repeat_ngram_size=int(no_repeat_ngram_size or 0))
+                                   no_repeat_ngram_size=int(no_repeat_ngram_size or 0), **steered)
             else:
                 p = SamplingParams(max_new_tokens=new, do_sample=True, temperature=temperature, top_k=top_k,
-                                   top_p=top_p, seed=seed + b,
+                                   top_p=top_p, seed=seed + b * made,
                                    eos_token_id=(eos_token_id if eos_token_id is not None
                                                  else getattr(self.config, 'eos_token_id', None)),
-                                   ban_eos=True, ignore_eos=True, no_repeat_ngram_size=int(no_repeat_ngram_size or 0))
+                                   ban_eos=True, ignore_eos=True, no_repeat_ngram_size=int(no_repeat_ngram_size or 0), **steered)
             params.append(p)
         engine.reset()
-        ids = [engine.add_request(toks, p) for toks, p in zip(rows, params)]
+        ids = [name for toks, p in zip(rows, params)
+               for name in (engine.add_samples(toks, p, made) if made > 1 else [engine.add_request(toks, p)])]
+        params = [p for p in params for _ in range(made)]
         column = 0              # generated tokens already handed to the streamer, the same for every row
         while engine.has_work:
             engine.step()
@@ -282,8 +337,13 @@ class CausalLMForSampling:
                 column += 1
         if streamer is not None:
             streamer.end()
-        result = torch.empty(len(rows), sequence_length, dtype=prompts.dtype)
-        result[:, :width] = prompts
+        if made > num_return_sequences:
+            families = [sorted(ids[b * made:(b + 1) * made], key=lambda i: -engine.requests[i].cumulative_logprob)[:num_return_sequences]
+                        for b in range(len(rows))]
+            ids = [i for family in families for i in family]
+            params = [engine.requests[i].params for i in ids]
+        result = torch.empty(len(ids), sequence_length, dtype=prompts.dtype)
+        result[:, :width] = prompts.repeat_interleave(num_return_sequences, 0)
         for b, i in enumerate(ids):
             out = engine.requests[i].output
             eos = params[b].eos_ids[0] if params[b].eos_ids else 0

@@ -100,20 +100,19 @@ class LLMEngine:
     def add_samples(self, prompt: Sequence[int], params: SamplingParams, count: int, req_id: Optional[Hashable] = None) -> List[Hashable]:
         """`count` requests for one prompt, each with a random stream of its own (the seeds that follow `params.seed`). The prompt is
         computed once, by the first of them, all but its newest token; the others take its pages over, where they are admitted while
-        it still runs. Their names: `req_id`, (`req_id`, 1), (`req_id`, 2) and so on."""
+        it still runs. Their names: `req_id`, (`req_id`, 1), (`req_id`, 2) and so on, or a number each where none is given."""
         if count < 1:
             raise ValueError(f"at least one sample is wanted, got {count}")
         if params.max_new_tokens < 1:
             raise ValueError("max_new_tokens must be at least 1")
-        rid = req_id if req_id is not None else next(self._ids)
-        names = [rid] + [(rid, i) for i in range(1, count)]
+        names = [next(self._ids) if req_id is None else (req_id, i) if i else req_id for i in range(count)]
         for name in names:
             if name in self.requests and not self.requests[name].finished:
                 raise ValueError(f"request {name!r} is already live")
         streams = [params] + [params if params.seed is None else dataclasses.replace(params, seed=params.seed + i) for i in range(1, count)]
         self._add(prompt, streams[0], names[0])
         for name, stream in zip(names[1:], streams[1:]):
-            self._add(prompt, stream, name, leader=self.requests[rid])
+            self._add(prompt, stream, name, leader=self.requests[names[0]])
         return names
 
     def fork_request(self, req_id: Hashable, params: Optional[SamplingParams] = None, new_id: Optional[Hashable] = None) -> Hashable:
@@ -233,7 +232,7 @@ class LLMEngine:
             if t is not None and not q.finished and q.mask is not None and (q.params.follows_grammar or q.params.no_repeat_ngram_size):
                 q.mask = self._mask(q)
                 if not q.mask.any():
-                    self.scheduler._end(q, "grammar", [])
+                    self.scheduler.end(q, "grammar")
         self.scheduler.finished.clear()        # the engine reports ends through `StepOutput`; nothing piles up
         if self.record_timings:
             self.runner.ops.synchronize()

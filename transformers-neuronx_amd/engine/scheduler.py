@@ -321,6 +321,10 @@ class Scheduler:
         self.finished.append(req)
         ended.append(req)
 
+    def end(self, req: Request, reason: str) -> None:
+        """The request is over behind the tokens it has."""
+        self._end(req, reason, [])
+
     def abort(self, req: Request) -> None:
         """Take a request out, wherever it stands: it ends with the reason "aborted" and gives back what it
         holds. A token that a step under way is still to deliver for it is dropped when it comes (`resolve`

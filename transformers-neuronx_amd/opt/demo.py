@@ -61,6 +61,11 @@ def _parser():
     run.add_argument("--top_p", type=float, default=1.0)
     run.add_argument("--temperature", type=float, default=1.0)
     run.add_argument("--no_repeat_ngram_size", type=int, default=0)
+    run.add_argument("--repetition_penalty", type=float, default=1.0)
+    run.add_argument("--frequency_penalty", type=float, default=0.0)
+    run.add_argument("--presence_penalty", type=float, default=0.0)
+    run.add_argument("--num_return_sequences", type=int, default=1, help="answers to each prompt")
+    run.add_argument("--best_of", type=int, default=None, help="answers made to each prompt, of which the likeliest are given")
     run.add_argument("--max_new_tokens", type=int, default=None)
     run.add_argument("--max_length", type=int, default=None)
     run.add_argument("--seed", type=int, default=15213)
@@ -102,7 +107,8 @@ def run(args):
         os.environ["TNX_SNAPSHOT_PATH"] = f"tnx_snapshot_{args.amp}_b{args.batch_size}"
         print(f"Set snapshot path {os.environ['TNX_SNAPSHOT_PATH']}")
     # the class is the one the folder's config.json names (OPT's, or that of any registered architecture)
-    model = NeuronAutoModelForCausalLM.from_pretrained(args.load, batch_size=args.batch_size, amp=args.amp,
+    answers = args.batch_size * max(args.num_return_sequences, args.best_of or 1)
+    model = NeuronAutoModelForCausalLM.from_pretrained(args.load, batch_size=answers, amp=args.amp,
                                                        tp_degree=args.tp_degree, n_positions=args.n_positions,
                                                        unroll=args.unroll,
                                                        context_length_estimate=args.context_length_estimate,
@@ -155,7 +161,9 @@ def run(args):
     def generate():
         return model.sample(input_ids, sequence_length=total, start_ids=start_ids, top_k=args.top_k,
                             temperature=args.temperature, top_p=args.top_p, seed=args.seed, generation_config=gen,
-                            no_repeat_ngram_size=args.no_repeat_ngram_size)
+                            no_repeat_ngram_size=args.no_repeat_ngram_size, repetition_penalty=args.repetition_penalty,
+                            frequency_penalty=args.frequency_penalty, presence_penalty=args.presence_penalty,
+                            num_return_sequences=args.num_return_sequences, best_of=args.best_of)
     out = generate()
     print("generated_sequence=", out)
     for i, logits in enumerate(dumped):
@@ -167,7 +175,7 @@ def run(args):
             print(f"Latency: {math.ceil(rec['seconds'] * 1000)} ms ({rec['tokens']} tokens)")
     if args.benchmark:
         model.engine.logits_hook = None
-        print(json.dumps(benchmark(model, generate, args.batch_size, input_ids.shape[1], total)))
+        print(json.dumps(benchmark(model, generate, answers, input_ids.shape[1], total)))
     if args.profile:
         from ..sampling.params import SamplingParams
         engine = model.engine
