@@ -216,7 +216,7 @@ class CacheManager:
     # ---------------------------------------------------------------- forks
 
     # Bytes of a run of places of which a part is worth copying alone. Values turned inside a page lie in runs of a line or two of memory:
-    # a part of such a line costs more than the whole (24 pages of 40 of 64 tokens' values in all layers of OPT-6.7b 168 us, whole 91).
+    # a part of such a line costs more than the whole (8 pages of 40 of 64 tokens' values to 24, all layers of OPT-6.7b: 147 us, whole 77).
     BOUNDED_RUN = 1024
 
     def _rows(self, group: str, bounded: bool):

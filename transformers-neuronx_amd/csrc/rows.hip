@@ -23,11 +23,10 @@ struct RowTensor {
 };
 
 #define ROW_THREADS 256
-#define ROW_UNITS 4           // units of a thread that are asked for together, before any is stored
 
 #define ROW_LINE 128          // bytes that memory is read by; a half of it is what it is written by at least
 
-// The first `bytes` (0 to 15) of `v`, and the rest of `w`.
+// The first `bytes` (0 to 16) of `v`, and the rest of `w`.
 __device__ __forceinline__ tnx_u32x4 joined(tnx_u32x4 v, tnx_u32x4 w, unsigned bytes) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
@@ -64,51 +63,34 @@ __device__ __forceinline__ void store_part(char* d, tnx_u32x4 v, unsigned bytes)
 //
 // FILL: what a run's last line lacks is filled up with what the target has there. Values turned inside a page are runs of 128 bytes,
 // of which a page that is not full moves a part; memory then reads, changes and writes back what it is given a part of. Values of 32
-// layers of 32 heads of 128, page 64, 8 pages to 24, in us: whole pages 91; 40 tokens (80 bytes of 128) parts 233, filled up 168;
-// 32 tokens (64 bytes) parts 70, filled up 195; 16 tokens 110 and 196. So lines are filled up where more than half of one is moved.
+// layers of 32 heads of 128, page 64, 8 pages to 24, in us: whole pages 77; 40 tokens (80 bytes of 128) parts 226, filled up 147; 32
+// tokens (64 bytes) parts 57, filled up 145; 20 tokens 106 and 151. So lines are filled up where more than half of one is moved.
 //
-// What bounds it is memory: stores are marked as not read again soon, which leaves the caches to the sources. 20 whole pages of
-// OPT-6.7b to 20 others, 0.67 GB read and as much written: 5.6 TB/s, 4.7 with plain stores, 5.3 with loads marked so too (as is right
-// for what fills up lines, 199 -> 168 us); one to eight units a thread asked for together are alike within 3%.
+// What bounds it is memory: stores are marked as not read again soon, which leaves the caches to the sources, a thread moves one unit,
+// and the blocks that run side by side are those of one tensor, whose rows lie nearest to one another. 20 whole pages of OPT-6.7b to 20
+// others, 0.67 GB read and as much written: 220 us, 6.1 TB/s (a large copy by the runtime 4.9); four units a thread 252, tensors side by
+// side 254, both 270; with plain stores 4.7 TB/s.
 template <typename V, bool FILL>
 __device__ __forceinline__ void copy_runs(const char* from, char* to, long long to_stride, const int* targets, int num_targets,
                                           long long stride, unsigned length, unsigned runs) {
   constexpr unsigned SIZE = sizeof(V);
   const unsigned wide = FILL ? (unsigned)min((long long)(length + ROW_LINE - 1) / ROW_LINE * ROW_LINE, stride) : length;
   const unsigned per_run = (wide + SIZE - 1) / SIZE, units = per_run * runs;
-  for (unsigned u0 = blockIdx.x * (ROW_THREADS * ROW_UNITS) + threadIdx.x; u0 < units; u0 += gridDim.x * (ROW_THREADS * ROW_UNITS)) {
-    V v[ROW_UNITS];
-    long long at[ROW_UNITS];
-    unsigned mine[ROW_UNITS];        // bytes of the unit that are the source's
-#pragma unroll
-    for (int k = 0; k < ROW_UNITS; ++k) {
-      const unsigned u = min(u0 + k * ROW_THREADS, units - 1);
-      const unsigned o = u / per_run, in = (u - o * per_run) * SIZE;
-      at[k] = o * stride + in;
-      mine[k] = in < length ? min(length - in, SIZE) : 0;
-      v[k] = *(const V*)(from + at[k]);
-    }
+  for (unsigned u = blockIdx.x * ROW_THREADS + threadIdx.x; u < units; u += gridDim.x * ROW_THREADS) {
+    const unsigned o = u / per_run, in = (u - o * per_run) * SIZE;
+    const unsigned mine = in < length ? min(length - in, SIZE) : 0;        // bytes of the unit that are the source's
+    const long long at = o * stride + in;
+    const V v = *(const V*)(from + at);
     for (int i = 0; i < num_targets; ++i) {
-      char* d = to + targets[i] * to_stride;
+      V* d = (V*)(to + targets[i] * to_stride + at);
       if constexpr (FILL) {
-        V w[ROW_UNITS];
-#pragma unroll
-        for (int k = 0; k < ROW_UNITS; ++k) {
-          w[k] = v[k];
-          if (mine[k] < SIZE) w[k] = __builtin_nontemporal_load((const V*)(d + at[k]));
-        }
-#pragma unroll
-        for (int k = 0; k < ROW_UNITS; ++k) {
-          if (mine[k] < SIZE) w[k] = joined(v[k], w[k], mine[k]);
-          if (u0 + k * ROW_THREADS < units) __builtin_nontemporal_store(w[k], (V*)(d + at[k]));
-        }
-      } else {
-#pragma unroll
-        for (int k = 0; k < ROW_UNITS; ++k) {
-          if (u0 + k * ROW_THREADS >= units) continue;
-          if (mine[k] == SIZE) __builtin_nontemporal_store(v[k], (V*)(d + at[k]));
-          else if constexpr (SIZE == 16) store_part(d + at[k], v[k], mine[k]);
-        }
+        V w = v;
+        if (mine < SIZE) w = __builtin_nontemporal_load(d);
+        __builtin_nontemporal_store(joined(v, w, mine), d);      // (one store for what a wave has of a line)
+      } else if (mine == SIZE) {
+        __builtin_nontemporal_store(v, d);
+      } else if constexpr (SIZE == 16) {
+        store_part((char*)d, v, mine);
       }
     }
   }
@@ -126,9 +108,9 @@ struct RowList {
 template <bool HERE>
 __global__ void __launch_bounds__(ROW_THREADS)
 copy_rows_kernel(const RowTensor* __restrict__ tensors, const RowList list, const int* __restrict__ far, int first_group, int num_groups) {
-  const RowTensor t = tensors[blockIdx.y];
+  const RowTensor t = tensors[blockIdx.z];
   const int* words = HERE ? list.words : far;
-  const int at = 4 * (first_group + (int)blockIdx.z);
+  const int at = 4 * (first_group + (int)blockIdx.y);
   const int4 g = make_int4(words[at], words[at + 1], words[at + 2], words[at + 3]);
   const char* from = t.from + g.x * t.from_stride;
   unsigned length = (unsigned)t.run, runs = (unsigned)t.outer;
@@ -154,14 +136,14 @@ extern "C" int tnx_copy_rows(const void* tensors, int num_tensors, const int* ho
   TNX_REQUIRE(num_tensors > 0 && num_tensors <= 65535 && num_groups > 0 && num_words > 4 * num_groups && units > 0 && units < (1ll << 31),
               "copy_rows: bad sizes tensors=%d groups=%d words=%d units=%lld", num_tensors, num_groups, num_words, units);
   TNX_REQUIRE(num_words <= ROW_WORDS ? host != nullptr : far != nullptr, "copy_rows: a list of %d words is missing", num_words);
-  const unsigned blocks = (unsigned)((units + ROW_THREADS * ROW_UNITS - 1) / (ROW_THREADS * ROW_UNITS));
+  const unsigned blocks = (unsigned)((units + ROW_THREADS - 1) / ROW_THREADS);
   RowList list;
   if (num_words <= ROW_WORDS) {
     for (int i = 0; i < num_words; ++i) list.words[i] = host[i];
     for (int i = num_words; i < ROW_WORDS; ++i) list.words[i] = 0;
   }
   for (int first = 0; first < num_groups; first += 65535) {
-    const dim3 grid(blocks, num_tensors, (unsigned)(num_groups - first < 65535 ? num_groups - first : 65535));
+    const dim3 grid(blocks, (unsigned)(num_groups - first < 65535 ? num_groups - first : 65535), num_tensors);
     if (num_words <= ROW_WORDS)
       copy_rows_kernel<true><<<grid, ROW_THREADS, 0, stream>>>((const RowTensor*)tensors, list, nullptr, first, num_groups);
     else
