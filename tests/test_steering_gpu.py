@@ -333,3 +333,18 @@ def test_refusals(ops):
         x.add_(1)
     assert ops.adjust_logits(x[:0], ops.logit_rules(40, rows=0)).shape == (0, 40)
     assert ops.log_probs(x[:0], tokens[:0], 2)[1].shape == (0, 2)
+
+
+def test_log_probs_sent_to_the_host(ops):
+    """Two on their way at a time, with and without alternatives."""
+    g = torch.Generator(device="cuda").manual_seed(6)
+    logits = torch.randn(5, 700, generator=g, device="cuda")
+    tokens = torch.randint(0, 700, (5,), generator=g, device="cuda").to(torch.int32)
+    for tops in ((0, 4), (4, 1), (9, 0)):
+        got = [ops.log_probs(logits, tokens, t) for t in tops]
+        sent = [ops.send_log_probs(*x) for x in got]
+        for x, s in zip(got, sent):
+            assert ops.receive_log_probs(s) == tuple(None if t is None else t.tolist() for t in x)
+    a = ops.log_probs(logits, tokens, 3)
+    with pytest.raises(ValueError):
+        ops.send_log_probs(a[0][:4], a[1], a[2])

@@ -396,3 +396,21 @@ extern "C" int tnx_log_probs(const float* logits, const int* tokens, float* out,
   TNX_CHECK_LAUNCH("log_probs");
   return 0;
 }
+
+// The log-probabilities, those of the alternatives and their tokens, one behind the other in pinned host memory.
+__global__ void send_log_probs_kernel(const int* __restrict__ out, const int* __restrict__ best, const int* __restrict__ ids, int rows,
+                                      int top, int* __restrict__ landing) {
+  const int i = blockIdx.x * blockDim.x + threadIdx.x, n = rows * top;
+  if (i < rows) landing[i] = out[i];
+  else if (i < rows + n) landing[i] = best[i - rows];
+  else if (i < rows + 2 * n) landing[i] = ids[i - rows - n];
+}
+
+extern "C" int tnx_send_log_probs(const float* out, const float* best, const int* ids, int rows, int top, int* landing, hipStream_t stream) {
+  TNX_REQUIRE(rows >= 0 && rows < (1 << 24) && top >= 0 && top <= SCORE_MOST_TOP && landing, "send_log_probs: bad sizes rows=%d top=%d", rows,
+              top);
+  if (rows == 0) return 0;
+  send_log_probs_kernel<<<(rows * (1 + 2 * top) + 255) / 256, 256, 0, stream>>>((const int*)out, (const int*)best, ids, rows, top, landing);
+  TNX_CHECK_LAUNCH("send_log_probs");
+  return 0;
+}

@@ -239,6 +239,7 @@ _SIGNATURES = {
         "tnx_start_history": [_c_void_p, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_void_p],
         "tnx_adjust_logits": [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_int,
                               _c_int, _c_void_p],
+        "tnx_send_log_probs": [_c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_void_p, _c_void_p],
         "tnx_log_probs": [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_void_p],
     },
     "probe": {
@@ -541,6 +542,7 @@ class HipOps:
         self._tiles_rooms = {}
         self._left_ways = {}
         self._landing, self._landing_turn = [None, None], 0
+        self._scores, self._scores_turn = [None, None], 0
         self._lost = self._ones_zeros = None
         self._ints, self._ints_done, self._ints_turn = [None, None], [None, None], 0
 
@@ -3050,19 +3052,31 @@ class HipOps:
         return out, ids, best
 
     def send_log_probs(self, out, ids, best):
-        """What `log_probs` gave, on its way to the host; `receive_log_probs` turns it into lists once it is there."""
-        landing = [None if t is None else torch.empty(t.shape, dtype=t.dtype, pin_memory=True) for t in (out, ids, best)]
-        for host, t in zip(landing, (out, ids, best)):
-            if t is not None:
-                host.copy_(t, non_blocking=True)
+        """What `log_probs` gave, on its way to the host by one launch; `receive_log_probs` turns it into lists once it is there. Two at
+        a time are on their way at most: a third takes the place of the first."""
+        rows, top = out.numel(), 0 if ids is None else ids.shape[1]
+        _want(out, "log-probabilities", torch.float32, (rows,))
+        if top:
+            _want(ids, "tokens", torch.int32, (rows, top))
+            _want(best, "their log-probabilities", torch.float32, (rows, top))
+        n = rows * (1 + 2 * top)
+        self._scores_turn ^= 1
+        pinned = self._scores[self._scores_turn]
+        if pinned is None or pinned[0].numel() < n:
+            pinned = self._scores[self._scores_turn] = self.pinned_ints(max(2 * n, 256))
+        self._call("steering", "tnx_send_log_probs", _ptr(out), _ptr(best), _ptr(ids), rows, top, pinned[1], _stream())
         landed = torch.cuda.Event()
         landed.record()
-        return landing, landed
+        return pinned[0], rows, top, landed
 
     def receive_log_probs(self, sent):
-        landing, landed = sent
+        host, rows, top, landed = sent
         landed.synchronize()
-        return tuple(None if t is None else t.tolist() for t in landing)
+        numbers = host.view(torch.float32)
+        if not top:
+            return numbers[:rows].tolist(), None, None
+        return (numbers[:rows].tolist(), host[rows * (1 + top):rows * (1 + 2 * top)].view(rows, top).tolist(),
+                numbers[rows:rows * (1 + top)].view(rows, top).tolist())
 
     def synchronize(self):
         torch.cuda.synchronize(self.device)
