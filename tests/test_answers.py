@@ -453,6 +453,14 @@ def test_params_that_are_refused(tiny_folders):
         with pytest.raises(ValueError):
             engine.add_samples([3], params, count)
     assert not engine.has_work and not engine.requests
+    calls = []
+
+    def refuses_the_third(output):
+        calls.append(output)
+        return [5] if len(calls) < 3 else []
+    with pytest.raises(ValueError, match="no token"):
+        engine.add_samples([3, 4], SamplingParams(allowed_tokens=refuses_the_third), 4, "q")
+    assert not engine.has_work and not engine.requests              # all of them or none
     engine.add_request([3], SamplingParams(), ("p", 1))
     with pytest.raises(ValueError, match="already live"):
         engine.add_samples([3], SamplingParams(), 2, "p")
@@ -526,6 +534,8 @@ def test_a_text_scored(tiny_folders, kernels):
     rows = prompts_of(cfg["vocab_size"], [30, 17], 5)
     ids = torch.zeros(2, 30, dtype=torch.long)
     ids[0], ids[1, 13:] = torch.tensor(rows[0]), torch.tensor(rows[1])
+    with pytest.raises(ValueError, match="vocabulary"):
+        model_of(folder, kernels).log_probs(torch.tensor([[3, cfg["vocab_size"]]]))
     for portion in (2048, 7):
         got = model_of(folder, kernels, max_num_batched_tokens=portion).log_probs(ids, start_ids=[0, 13])
         for b, toks in enumerate(rows):

@@ -60,7 +60,8 @@ def test_sets_of_rows_that_are_refused():
     for bad in (dict(tensors=[]), dict(tensors=[t], token_axes=[0]), dict(tensors=[t], token_axes=[3]),
                 dict(tensors=[t.transpose(1, 2)]), dict(tensors=[t, torch.zeros(6, 4, 16)], token_axes=[2, 2]),
                 dict(tensors=[t], targets=[t.double()]), dict(tensors=[t], targets=[torch.zeros(6, 8, 4)]),
-                dict(tensors=[t, t], token_axes=[1]), dict(tensors=[torch.zeros(0, 3)]), dict(tensors=[torch.zeros(1, 4).expand(3, 4)])):
+                dict(tensors=[t, t]), dict(tensors=[t[:3]], targets=[t[2:]]), dict(tensors=[t[:, :2], t[:, 2:]]),
+                dict(tensors=[t, torch.zeros(6, 3)], token_axes=[1]), dict(tensors=[torch.zeros(0, 3)]), dict(tensors=[torch.zeros(1, 4).expand(3, 4)])):
         with pytest.raises(ValueError):
             RowSet(**bad)
     with pytest.raises(ValueError, match="counts tokens"):
@@ -138,3 +139,13 @@ def test_log_probs_of_rows_with_infinities():
     assert got.tolist() == [-inf, pytest.approx(-math.log(2)), 0.0, -inf, -inf]
     assert ids.tolist() == [[0, 1, 2], [0, 2, 1], [1, 0, 2], [0, 1, 2], [0, 1, 2]]
     assert best[0].tolist() == [-inf] * 3 and best[1].tolist()[2] == -inf and best[3].tolist() == [pytest.approx(-math.log(2))] * 2 + [-inf]
+
+
+def test_a_full_history_and_tokens_of_no_vocabulary_on_the_host():
+    """A history without room takes no further token; entries and tokens outside the vocabulary touch nothing."""
+    entries = torch.tensor([[[0, 2], [1, 2]], [[50, 2], [-3, 2]]], dtype=torch.int32)
+    history = TokenHistory(entries.clone(), torch.tensor([2, 2], dtype=torch.int32))
+    logits = torch.ones(2, 4)
+    rules = OPS.logit_rules(4, slots=[0, 1], presence=[0.5, 0.5])
+    OPS.adjust_logits(logits, rules, history, torch.tensor([3, 99], dtype=torch.int32))
+    assert logits.tolist() == [[0.5, 0.5, 1, 1], [1, 1, 1, 1]] and torch.equal(history.entries, entries) and history.used.tolist() == [2, 2]

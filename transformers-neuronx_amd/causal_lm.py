@@ -242,6 +242,9 @@ class CausalLMForSampling:
         out = torch.zeros(len(rows), torch.as_tensor(input_ids).shape[-1])
         portion = self.engine_config.max_num_batched_tokens
         for b, toks in enumerate(rows):
+            if toks and not 0 <= min(toks) <= max(toks) < runner.vocab:
+                raise ValueError(f"row {b}: a token id is outside the vocabulary of {runner.vocab}")
+        for b, toks in enumerate(rows):
             key = ("scored", b)
             try:
                 for at in range(0, len(toks) - 1, portion):

@@ -110,9 +110,13 @@ class LLMEngine:
             if name in self.requests and not self.requests[name].finished:
                 raise ValueError(f"request {name!r} is already live")
         streams = [params] + [params if params.seed is None else dataclasses.replace(params, seed=params.seed + i) for i in range(1, count)]
-        self._add(prompt, streams[0], names[0])
-        for name, stream in zip(names[1:], streams[1:]):
-            self._add(prompt, stream, name, leader=self.requests[names[0]])
+        for i, (name, stream) in enumerate(zip(names, streams)):
+            try:
+                self._add(prompt, stream, name, leader=self.requests[names[0]] if i else None)
+            except Exception:
+                for added in names[:i]:                # all of them or none
+                    self.abort_request(added)
+                raise
         return names
 
     def fork_request(self, req_id: Hashable, params: Optional[SamplingParams] = None, new_id: Optional[Hashable] = None) -> Hashable:

@@ -56,10 +56,10 @@ class Request:
     # The request whose pages this one takes its first `shared` tokens from, where it still can when it is admitted: all that both had
     # when this one was made but the newest, which it brings itself, to choose a token of its own from. The leader's portion ends there
     # too, for those waiting for it.
-    leader: Optional["Request"] = None
+    leader: Optional["Request"] = field(default=None, repr=False)
     shared: int = 0
-    followers: List["Request"] = field(default_factory=list)      # that wait for this one
-    mask: Optional[object] = None   # the tokens that may be chosen next (`pack_mask`); None: all
+    followers: List["Request"] = field(default_factory=list, repr=False)      # that wait for this one
+    mask: Optional[object] = field(default=None, repr=False)   # the tokens that may be chosen next (`pack_mask`); None: all
     history_of: Optional[tuple] = None      # the (slot, preemptions) under which the device keeps its history
     # of every token of the output, where the request asks for them
     logprobs: List[float] = field(default_factory=list)

@@ -2895,8 +2895,9 @@ class HipOps:
         """Launches go to the current device's stream: what they work on lies there."""
         if device.type != "cuda":
             raise ValueError(f"{what} must be on the GPU")
-        if device.index != torch._C._cuda_getDevice():
-            raise ValueError(f"{what} on {device}, but the current device is cuda:{torch._C._cuda_getDevice()}")
+        at = torch._C._cuda_getDevice()
+        if device.index != at or self.device.index not in (None, at):
+            raise ValueError(f"{what} on {device}, but the current device is cuda:{at} and these kernels work on {self.device}")
 
     def _from_host(self, flat, what):
         """`send_ints` for what is made of the host's lists: not while a graph is recorded, whose replays would read what the

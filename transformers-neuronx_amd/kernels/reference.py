@@ -1039,10 +1039,12 @@ class ReferenceOps:
                     at = (history.entries[slot, :n, 0] == token).nonzero().flatten()
                     if at.numel():
                         history.entries[slot, at[0], 1] += 2
-                    else:
+                    elif n < history.capacity and token < rules.vocab:
                         history.entries[slot, n] = torch.tensor([token, 2], dtype=torch.int32)
                         history.used[slot] = n = n + 1
                 ids, info = history.entries[slot, :n, 0].long(), history.entries[slot, :n, 1]
+                there = (ids >= 0) & (ids < rules.vocab)
+                ids, info = ids[there], info[there]
                 rho, presence, frequency = (float(v) for v in numbers[i])
                 times = (info >> 1).float()
                 x = row[ids]

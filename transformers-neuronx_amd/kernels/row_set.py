@@ -13,6 +13,8 @@ class RowSet:
                  tensor whose rows are always copied whole; left out: None for all
     targets      the tensors that rows are copied to, of the same types and shapes but for the number of rows; left out: the
                  tensors themselves
+
+    No two of them lie in the same memory: what is copied would depend on which is copied first.
     """
 
     def __init__(self, tensors: Sequence[torch.Tensor], token_axes: Optional[Sequence[Optional[int]]] = None,
@@ -53,6 +55,10 @@ class RowSet:
             distances = [t.data_ptr(), to.data_ptr(), run] + [x.stride(0) * item for x in (t, to) if x.shape[0] > 1]
             grain = next(g for g in (16, 4, 2, 1) if all(d % g == 0 for d in distances + ([] if g == 16 else [inner])))
             words.append([t.data_ptr(), to.data_ptr(), t.stride(0) * item, to.stride(0) * item, run, inner, outer, grain])
+        spans = sorted((x.data_ptr(), x.data_ptr() + ((x.shape[0] - 1) * x.stride(0) + x[0].numel()) * x.element_size())
+                       for x in (self.tensors if self.in_place else self.tensors + self.targets))
+        if any(end > begin for (_, end), (begin, _) in zip(spans, spans[1:])):
+            raise ValueError("two tensors of a set of rows share memory")
         if len(places) > 1:
             raise ValueError(f"the token axes of a set of rows are of one length, got {sorted(places)}")
         self.places: Optional[int] = places.pop() if places else None
