@@ -262,6 +262,54 @@ def test_log_probs_of_rows_with_infinities(ops, vocab):
     _check_log_probs(logits, tokens, top, ops.log_probs(logits, tokens, top))
 
 
+@pytest.mark.parametrize("vocab", [60, 20001])
+def test_log_probs_of_values_far_out(ops, vocab):
+    """Rows whose values, or some of them, lie where powers overflow, and sums of very many alike."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.randn(10, vocab, generator=g, device="cuda")
+    low = torch.finfo(torch.float32).min
+    x[0] = low
+    x[1, ::2] = low
+    x[2, 1:] = low
+    x[3] = x[3].abs() * 1e37
+    x[4] = -x[4].abs() * 3e38
+    x[5] = -1e31 + x[5] * 1e25
+    x[6] = 1000 + x[6]
+    x[7] = -3e4 + x[7] * 300
+    x[8, 5] = 3e38
+    x[9] = x[9] * 1e-30
+    tokens = torch.randint(0, vocab, (10,), generator=g, device="cuda").to(torch.int32)
+    got = ops.log_probs(x, tokens, 3)
+    want, ids, best = log_probs_in_64(x.cpu().numpy(), tokens.cpu().numpy(), 3)
+    steps = 8 + np.log2(vocab) + vocab / 256
+    for a, b in ((got[0], want), (got[2], best)):
+        a = a.cpu().numpy().astype(np.float64)
+        with np.errstate(over="ignore"):
+            b = b.astype(np.float32).astype(np.float64)         # a difference of two lowest values overflows
+        fine = np.isfinite(b)
+        assert np.array_equal(fine, np.isfinite(a))
+        # beside the sum's own error the difference of a logit and the largest is rounded once, and both count by their size
+        assert (np.abs(a[fine] - b[fine]) <= steps * 2.0 ** -24 * (1 + np.abs(b[fine]))).all()
+    assert np.array_equal(got[1].cpu().numpy(), ids)
+
+
+def test_log_probs_beyond_two_to_the_31_elements(ops):
+    rows, vocab = 43000, 50001
+    logits = torch.empty(rows, vocab, device="cuda")
+    logits[-3:].normal_(generator=torch.Generator(device="cuda").manual_seed(5))
+    logits[:-3].fill_(1.0)
+    tokens = torch.arange(rows, device="cuda", dtype=torch.int32) % vocab
+    got = ops.log_probs(logits, tokens, 2)
+    _check_log_probs(logits[-3:], tokens[-3:], 2, [t[-3:] for t in got])
+    assert torch.allclose(got[0][:-3], torch.full((1,), -np.log(vocab), device="cuda").float(), atol=1e-4)
+    rules = ops.logit_rules(vocab, rows=rows, biases=[None] * (rows - 1) + [{vocab - 1: 5.0, 0: float("-inf")}])
+    before = logits[-1].clone()
+    ops.adjust_logits(logits, rules)
+    before[vocab - 1] += 5.0
+    before[0] = float("-inf")
+    assert torch.equal(logits[-1], before) and (logits[-4] == 1).all()
+
+
 def test_log_probs_of_a_part_and_in_a_graph(ops):
     g = torch.Generator(device="cuda").manual_seed(4)
     whole = torch.randn(4 * 999 + 3, generator=g, device="cuda")

@@ -181,33 +181,48 @@ __device__ __forceinline__ float key_value(unsigned long long key) {
   return __uint_as_float((u & 0x80000000u) ? u & 0x7FFFFFFFu : ~u);
 }
 
-// exp(d) for d <= 0 by the hardware's power of two; log2(e) in two parts, so that only the roundings of d and of the power's argument
-// are left: 2^-24 of |d| each, and what is far below the largest adds little.
-__device__ __forceinline__ float exp_of(float d) {
-  const float hi = 1.44269502162933349609375f, lo = 1.92596299112661746887e-8f;
-  return __builtin_amdgcn_exp2f(fmaf(d, hi, d * lo));
-}
+// log2(e) in two parts, of which the second is what the first lacks
+#define LOG2E_HI 1.44269502162933349609375f
+#define LOG2E_LO 1.92596299112661746887e-8f
+// exp(d) for d <= 0 by the hardware's power of two: the roundings of d and of the power's argument are left, 2^-24 of |d| each.
+__device__ __forceinline__ float exp_of(float d) { return __builtin_amdgcn_exp2f(fmaf(d, LOG2E_HI, d * LOG2E_LO)); }
+
+// exp(x - r) for many x and one r is 2^(x log2(e) - r log2(e)): one multiply-add and the power an element, with the product of r
+// rounded, and what the rounding lost put back behind the sum. Left is the rounding of the power's argument, and 1.3e-8 of x - r for
+// what the constant lacks.
+struct PowersBelow {
+  float r, shift, lost;
+  __device__ __forceinline__ void at(float reference) {
+    r = reference;
+    shift = -(r * LOG2E_HI);
+    lost = fmaf(-r, LOG2E_HI, -shift);
+  }
+  __device__ __forceinline__ float operator()(float x) const { return __builtin_amdgcn_exp2f(fmaf(x, LOG2E_HI, shift)); }
+  __device__ __forceinline__ float back() const { return __builtin_amdgcn_exp2f(lost); }
+};
+// Beyond this many powers overflow on the way; rows with such a maximum are summed again with care.
+#define SCORE_FAR 1e30f
 
 // A row read four logits at a time from the boundary of 16 bytes at or before it: quad q holds elements 4 q - lead to 4 q - lead + 3;
-// what lies outside the row reads as -inf. A NaN reads as -inf as well.
+// what lies outside the row reads as -inf.
 struct Quads {
   const float* row;
   int vocab, lead, count;
   __device__ __forceinline__ Quads(const float* r, int v)
       : row(r), vocab(v), lead((int)(((uintptr_t)r >> 2) & 3)), count((v + (int)(((uintptr_t)r >> 2) & 3) + 3) / 4) {}
   __device__ __forceinline__ int first(int q) const { return 4 * q - lead; }
-  template <bool ONCE = false>
+  __device__ __forceinline__ bool whole(int q) const { return 4 * q - lead >= 0 && 4 * q - lead + 3 < vocab; }
+  template <bool ONCE>
+  __device__ __forceinline__ f32x4 inside(int q) const {
+    const f32x4* p = (const f32x4*)(row + 4 * q - lead);
+    return ONCE ? __builtin_nontemporal_load(p) : *p;
+  }
   __device__ __forceinline__ f32x4 operator()(int q) const {
+    if (whole(q)) return inside<false>(q);
     const int i = 4 * q - lead;
     f32x4 x;
-    if (i >= 0 && i + 3 < vocab) {
-      x = ONCE ? __builtin_nontemporal_load((const f32x4*)(row + i)) : *(const f32x4*)(row + i);
-    } else {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = q < count && i + e >= 0 && i + e < vocab ? row[i + e] : -INFINITY;
-    }
-#pragma unroll
-    for (int e = 0; e < 4; ++e) x[e] = fmaxf(x[e], -INFINITY);
+    for (int e = 0; e < 4; ++e) x[e] = i + e >= 0 && i + e < vocab ? row[i + e] : -INFINITY;
     return x;
   }
 };
@@ -223,6 +238,10 @@ struct Quads {
 // the logits of these groups are looked at again, and those of them that are no smaller than the last group's best, hardly more than
 // the alternatives themselves, are ranked in LDS. Should they be more than fit (the best of a long row all in a few threads' places),
 // the alternatives are found one by one, each with a pass of its own.
+//
+// Many rows are bound by memory. A few are bound by what one compute unit can do: a row of 50,272 takes 5.7 us without and 9.4 with
+// alternatives, of which 2.6 are those of any launch, about 3 the powers and maxima, and the rest five barriers with a trip through
+// LDS or memory each. (Rows held in registers, all asked for at once: 7.3 and 17. Groups of 128 for 256, 2 keys a read: 4 us of 6.)
 template <int THREADS, bool TOP, bool ONCE>
 __global__ void __launch_bounds__(THREADS)
 log_probs_kernel(const float* __restrict__ logits, const int* __restrict__ tokens, float* __restrict__ out, int* __restrict__ top_tokens,
@@ -234,19 +253,20 @@ log_probs_kernel(const float* __restrict__ logits, const int* __restrict__ token
   const float* row = quads.row;
 
   float m = -INFINITY, s = 0.f;
-  int at = quads.first(tid);          // where the thread's largest logit came first
-  if (at < 0) at = 0;
-  for (int q0 = tid; q0 < quads.count; q0 += 4 * THREADS) {
-    f32x4 v[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] = quads.template operator()<ONCE>(q0 + k * THREADS);
-    float here = v[0][0];
+  int at = max(quads.first(tid), 0);          // where the thread's largest logit came first
+  PowersBelow power;
+  power.at(-SCORE_FAR);
+  auto take = [&](const f32x4 (&v)[4], int q0) __attribute__((always_inline)) {
+    float here = v[0][0];                     // (the larger of a number and a NaN is the number)
 #pragma unroll
     for (int k = 0; k < 4; ++k)
 #pragma unroll
       for (int e = 0; e < 4; ++e) here = fmaxf(here, v[k][e]);
     if (here > m) {
-      s *= m > -INFINITY ? exp_of(m - here) : 0.f;
+      PowersBelow next;
+      next.at(fmaxf(here, -SCORE_FAR));
+      s *= __builtin_amdgcn_exp2f(fmaf(power.r - next.r, LOG2E_HI, power.lost - next.lost));
+      power = next;
       m = here;
       if constexpr (TOP) {
 #pragma unroll
@@ -255,11 +275,23 @@ log_probs_kernel(const float* __restrict__ logits, const int* __restrict__ token
           for (int e = 3; e >= 0; --e) at = v[k][e] == here ? quads.first(q0 + k * THREADS) + e : at;
       }
     }
-    const float base = fmaxf(m, -3.402823466e38f);       // -inf less -inf would be no number
+    float part[2] = {0.f, 0.f};
 #pragma unroll
     for (int k = 0; k < 4; ++k)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s += exp_of(v[k][e] - base);
+      for (int e = 0; e < 4; ++e) part[e & 1] += power(v[k][e]);
+    s += part[0] + part[1];
+  };
+  for (int b = 0; b < quads.count; b += 4 * THREADS) {
+    f32x4 v[4];
+    if (quads.whole(b) && quads.whole(b + 4 * THREADS - 1)) {         // the same for all threads
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[k] = quads.template inside<ONCE>(b + tid + k * THREADS);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[k] = quads(b + tid + k * THREADS);
+    }
+    take(v, b + tid);
   }
   const float mine = m;
   m = wave_max(m);
@@ -268,24 +300,26 @@ log_probs_kernel(const float* __restrict__ logits, const int* __restrict__ token
   m = scratch[0];
 #pragma unroll
   for (int w = 1; w < WAVES; ++w) m = fmaxf(m, scratch[w]);
-  if (m < INFINITY) {
-    s = mine > -INFINITY ? s * exp_of(mine - m) : 0.f;
-  } else {                            // those at +inf are counted
-    s = 0.f;
+  s = block_sum<WAVES>(s * power.back() * exp_of(power.r - m), sums);
+  if (!(s < INFINITY) || !(fabsf(m) < SCORE_FAR)) {
+    // with a NaN somewhere, or a maximum that is far out or none: one by one
+    float exact = 0.f;
     for (int q = tid; q < quads.count; q += THREADS) {
       const f32x4 x = quads(q);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s += x[e] == INFINITY ? 1.f : 0.f;
+      for (int e = 0; e < 4; ++e) exact += x[e] > -INFINITY ? (x[e] == m ? 1.f : exp_of(x[e] - m)) : 0.f;
     }
+    s = block_sum<WAVES>(exact, sums);
   }
-  const float log_l = logf(block_sum<WAVES>(s, sums));
+  const float log_l = logf(s);
   if (tid == 0) {
     const int t = tokens[blockIdx.x];
     out[blockIdx.x] = t >= 0 && t < vocab ? log_prob_of(row[t], m, log_l) : -INFINITY;
   }
   if constexpr (TOP) {
-    __shared__ unsigned long long best[SCORE_GROUPS], gathered[SCORE_GATHER], one[WAVES];
-    __shared__ int winners[SCORE_MOST_TOP], num_winners, num_gathered;
+    __shared__ __align__(16) unsigned long long best[SCORE_GROUPS];
+    __shared__ unsigned long long gathered[SCORE_GATHER], one[WAVES];
+    __shared__ int winners[SCORE_MOST_TOP], num_gathered;
     __shared__ unsigned long long least;
     // the thread's best as a key (its logit, then the lower token id), and its group's
     unsigned long long key = tid < quads.count ? order_key(mine, at) : 0;
@@ -296,27 +330,32 @@ log_probs_kernel(const float* __restrict__ logits, const int* __restrict__ token
     }
     if (tid % PER_GROUP == 0) best[tid / PER_GROUP] = key;
     if (tid == 0) {
-      num_winners = num_gathered = 0;
+      num_gathered = 0;
       least = 0;
     }
     __syncthreads();
-    if (tid < SCORE_GROUPS && best[tid] != 0) {          // (0: a group without logits)
+    const int groups = (min(quads.count, THREADS) + PER_GROUP - 1) / PER_GROUP;      // that have logits; the others' keys are 0
+    if (tid < groups) {
       const unsigned long long b = best[tid];
       int rank = 0;
-      for (int j = 0; j < SCORE_GROUPS; ++j) rank += best[j] > b ? 1 : 0;
-      if (rank < top) {
-        winners[rank] = tid;
-        atomicAdd(&num_winners, 1);
+#pragma unroll 8
+      for (int j = 0; j < SCORE_GROUPS; j += 2) {
+        const ulonglong2 two = *(const ulonglong2*)&best[j];
+        rank += (two.x > b ? 1 : 0) + (two.y > b ? 1 : 0);
       }
+      if (rank < top) winners[rank] = tid;
       if (rank == top - 1) least = b;                    // (fewer groups than alternatives: everything is gathered)
     }
     __syncthreads();
     // group g's quads are those of its threads: k * THREADS + PER_GROUP * g + j
     const int rounds = (quads.count + THREADS - 1) / THREADS * PER_GROUP;
     const unsigned long long floor_key = least;
-    for (int w = wave; w < num_winners; w += WAVES)
-      for (int n = lane; n < rounds; n += 64) {
-        const int q = n / PER_GROUP * THREADS + PER_GROUP * winners[w] + n % PER_GROUP;
+    // a wave takes 64 of them at a time
+    const int parts = (rounds + 63) / 64;
+    for (int item = wave; item < min(top, groups) * parts; item += WAVES) {
+      const int n = item % parts * 64 + lane;
+      if (n < rounds) {
+        const int q = n / PER_GROUP * THREADS + PER_GROUP * winners[item / parts] + n % PER_GROUP;
         const f32x4 x = quads(q);
         const int i = quads.first(q);
 #pragma unroll
@@ -329,6 +368,7 @@ log_probs_kernel(const float* __restrict__ logits, const int* __restrict__ token
             }
           }
       }
+    }
     __syncthreads();
     const int n = num_gathered;
     int* ids = top_tokens + (size_t)blockIdx.x * top;
@@ -385,10 +425,10 @@ extern "C" int tnx_log_probs(const float* logits, const int* tokens, float* out,
               "log_probs: bad sizes rows=%d vocab=%d top=%d", rows, vocab, top);
   if (rows == 0) return 0;
   // 1,024 threads where each has a whole round of 16 logits and the rows are no more than the blocks that run at once, 512 otherwise.
-  // In us, 1,024 / 512 / 256 threads: 64 rows of 50,272 with 20 alternatives 13.9 / 18.9 / 29.7, 512 rows 25.4 / 28.4 / 42.7, 777 rows
-  // 45.5 / 39.4 / 51.2; 64 rows of 5,000 with 5 7.1 / 6.4 / 7.5, 2,048 rows 29.4 / 18.3 / 18.0.
-  // Rows that the caches cannot hold are marked as read once: 2,048 rows of 50,272 without alternatives 65.8 us (6.3 TB/s), 73.5 plain,
-  // 2,048 of 32,001 44.0 and 48.4; but 777 of 32,001 (99 MB) with 20 27.6 and 26.1, 64 of 50,272 10.6 and 8.6.
+  // In us, 1,024 / 512: 64 rows of 50,272 with 20 alternatives 11.9 / 14.0, 512 rows 25.0 / 26.4, 777 rows 40.9 / 40.2; 64 rows of
+  // 32,001 with 5 9.5 / 10.3, of 12,000 7.1 / 7.2, of 5,000 7.0 / 6.4, 2,048 rows of 5,000 29.3 / 18.7.
+  // Rows that the caches cannot hold are marked as read once: 2,048 rows of 50,272 without alternatives 62.3 us (6.6 TB/s), 70.9 plain,
+  // 2,048 of 32,001 41.8 and 46.6; but 777 of 32,001 (99 MB) with 20 28.6 and 27.5, 64 of 50,272 16.9 and 14.0.
   const bool once = (long long)rows * vocab * 4 >= (128ll << 20);
   if (rows <= 512 && vocab >= 16 * 1024) launch_log_probs<1024, false>(logits, tokens, out, top_tokens, top_out, top, rows, vocab, stream);
   else if (once) launch_log_probs<512, true>(logits, tokens, out, top_tokens, top_out, top, rows, vocab, stream);
