@@ -212,6 +212,36 @@ def test_forks_that_are_refused():
         m.resize(0)
 
 
+def test_a_cache_that_finds_no_memory_halfway_stays_whole(monkeypatch):
+    for size in (60, 12):
+        m = manager(num_pages=20, window=None)
+        for name, n in (("a", 20), ("b", 35), ("c", 7)):
+            m.add_request(name)
+            m.grow(name, n)
+            fill(m, name, 0, list(range(1, n + 1)))
+            m.advance(name, n)
+        m.free_request("a")
+        new, made = m._new_pages, []
+
+        def fails_the_second_time(need, num_pages):
+            made.append(num_pages)
+            if len(made) == 2:
+                raise MemoryError
+            return new(need, num_pages)
+        monkeypatch.setattr(m, "_new_pages", fails_the_second_time)
+        with pytest.raises(MemoryError):
+            m.resize(size)
+        m.check()
+        assert m.groups["full"].pool.num_pages == min(size, 20)
+        holds(m, "b", list(range(1, 36)))
+        holds(m, "c", list(range(1, 8)))
+        m.fork("b", "d")
+        m.resize(size)
+        assert {len(m.caches[c].pages["k"]) for c in (0, 1)} == {size}
+        for name in ("b", "d"):
+            holds(m, name, list(range(1, 36)))
+
+
 # ---------------------------------------------------------------- answers that share a prompt
 
 @BOTH
@@ -525,6 +555,17 @@ def test_sequences_from_the_entry_point(tiny_folders, kernels):
     for bad in (dict(num_return_sequences=0), dict(num_return_sequences=3, best_of=2)):
         with pytest.raises(ValueError):
             model.sample(ids, 18, **bad)
+
+
+@pytest.mark.gpu
+def test_the_command_line(tiny_folders, capsys, tmp_path):
+    from transformers_neuronx_amd.opt.demo import main
+    folder, cfg, _ = tiny_folders["A"]
+    main(["--amp", "f32", "run", folder, "--batch_size", "2", "--n_positions", "32", "--prompt_len", "9", "--max_new_tokens", "6", "--do_sample",
+          "--top_k", "30", "--num_return_sequences", "2", "--best_of", "3", "--repetition_penalty", "1.2", "--frequency_penalty", "0.1",
+          "--presence_penalty", "0.1", "--dump_logits", str(tmp_path / "d"), "--dump_logits_limit", "-1"])
+    out = capsys.readouterr().out
+    assert out.count("[") >= 5 and "Dumped the logits of" in out
 
 
 @BOTH

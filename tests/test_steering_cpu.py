@@ -111,7 +111,8 @@ def test_masks():
     assert mask_words(33) == 2
     assert pack_mask(33, [0, 31, 32]).tolist() == [1 | -2 ** 31, 1]
     assert pack_mask(33, np.arange(33) == 32).tolist() == [0, 1]
-    for bad in ([33], [-1], np.ones(32, dtype=bool)):
+    assert pack_mask(33, {32, 0}).tolist() == [1, 1] and pack_mask(33, range(3)).tolist() == [7, 0] and not pack_mask(33, []).any()
+    for bad in ([33], [-1], np.ones(32, dtype=bool), [1.5], ["a"]):
         with pytest.raises(ValueError):
             pack_mask(33, bad)
 

@@ -62,8 +62,10 @@ __device__ __forceinline__ float penalised(float x, const RowRules& r, int info)
 // ADJUST_THREADS * ADJUST_BARRED logits each. A logit is written by one thread at a time: history entries name distinct tokens,
 // so do a row's biases, a barrier lies between the two, and barred tokens are left to the other blocks, which write nothing else.
 //
-// Of a row's logits only those named are read, and only those barred written: what bounds a batch without masks is the way from the
-// rules to the history's entries, to the logits and back, three trips to memory one behind the other, not their bytes.
+// Of a row's logits only those named are read, and only those barred written: what bounds a batch is the way from the rules to the
+// history's entries, to the logits and back, and to the biases' logits and back, trips to memory one behind the other, not their bytes.
+// One row with 120 entries 2.2 us, 64 rows of 50,272 with 1,500 entries and 300 biases 6.7, with half of the tokens barred as well 9.2;
+// half of the tokens barred alone 6.6 (one logit a lane, so that a wave's stores lie side by side; four a lane 10.4).
 __global__ void __launch_bounds__(ADJUST_THREADS)
 adjust_logits_kernel(float* __restrict__ logits, const RowRules* __restrict__ rules, const int* __restrict__ bias_tokens,
                      const float* __restrict__ bias_values, int2* __restrict__ entries, int* __restrict__ used, int capacity,

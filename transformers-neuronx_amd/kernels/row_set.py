@@ -1,4 +1,5 @@
 """Rows of several tensors that are copied together: what a page (or a slot) is across all layers of a cache."""
+import math
 from typing import List, Optional, Sequence, Tuple
 
 import numpy as np
@@ -28,35 +29,31 @@ class RowSet:
         if not len(self.tensors) == len(self.token_axes) == len(self.targets):
             raise ValueError(f"{len(self.tensors)} tensors, {len(self.token_axes)} token axes, {len(self.targets)} targets")
         self.device = self.tensors[0].device
-        words, places = [], set()
+        words, places, spans = [], set(), []
         for t, axis, to in zip(self.tensors, self.token_axes, self.targets):
-            for x in (t, to):
-                if x.device != self.device:
-                    raise ValueError(f"the tensors of a set of rows lie on one device, got {self.device} and {x.device}")
-                if x.dim() < 1 or x.numel() == 0:
-                    raise ValueError(f"a set of rows takes tensors with rows in them, got shape {tuple(x.shape)}")
-                if not x[0].is_contiguous() or (x.shape[0] > 1 and x.stride(0) < x[0].numel()):
-                    raise ValueError("a row has to be contiguous, and rows may not overlap")
-            if to.dtype != t.dtype or to.shape[1:] != t.shape[1:]:
-                raise ValueError(f"rows of {t.dtype} {tuple(t.shape[1:])} cannot go to rows of {to.dtype} {tuple(to.shape[1:])}")
-            item, shape = t.element_size(), list(t.shape)
-            row = int(np.prod(shape[1:], dtype=np.int64)) * item
+            at, apart, shape, item = self._layout(t)
+            to_at, to_apart, to_shape, _ = (at, apart, shape, item) if to is t else self._layout(to)
+            if to.dtype != t.dtype or to_shape[1:] != shape[1:]:
+                raise ValueError(f"rows of {t.dtype} {shape[1:]} cannot go to rows of {to.dtype} {to_shape[1:]}")
+            row = math.prod(shape[1:]) * item
             if row >= 2 ** 31:
                 raise ValueError(f"a row of {row} bytes is more than copy_rows takes (2 GiB)")
             if axis is None:
                 run, inner, outer = row, 0, 1
             else:
-                if not 0 < axis < t.dim():
-                    raise ValueError(f"the token axis of a tensor of shape {tuple(t.shape)} is one of 1 to {t.dim() - 1}, got {axis}")
-                inner = int(np.prod(shape[axis + 1:], dtype=np.int64)) * item
+                if not 0 < axis < len(shape):
+                    raise ValueError(f"the token axis of a tensor of shape {shape} is one of 1 to {len(shape) - 1}, got {axis}")
+                inner = math.prod(shape[axis + 1:]) * item
                 run = shape[axis] * inner
                 outer = row // run
                 places.add(shape[axis])
-            distances = [t.data_ptr(), to.data_ptr(), run] + [x.stride(0) * item for x in (t, to) if x.shape[0] > 1]
-            grain = next(g for g in (16, 4, 2, 1) if all(d % g == 0 for d in distances + ([] if g == 16 else [inner])))
-            words.append([t.data_ptr(), to.data_ptr(), t.stride(0) * item, to.stride(0) * item, run, inner, outer, grain])
-        spans = sorted((x.data_ptr(), x.data_ptr() + ((x.shape[0] - 1) * x.stride(0) + x[0].numel()) * x.element_size())
-                       for x in (self.tensors if self.in_place else self.tensors + self.targets))
+            distances = at | to_at | run | (apart if shape[0] > 1 else 0) | (to_apart if to_shape[0] > 1 else 0)
+            grain = next(g for g in (16, 4, 2, 1) if distances % g == 0 and (g == 16 or inner % g == 0))
+            words.append((at, to_at, apart, to_apart, run, inner, outer, grain))
+            spans.append((at, at + (shape[0] - 1) * apart + row))
+            if not self.in_place:
+                spans.append((to_at, to_at + (to_shape[0] - 1) * to_apart + row))
+        spans.sort()
         if any(end > begin for (_, end), (begin, _) in zip(spans, spans[1:])):
             raise ValueError("two tensors of a set of rows share memory")
         if len(places) > 1:
@@ -68,6 +65,22 @@ class RowSet:
         self._shapes = sorted({tuple(w[4:]) for w in words})
         self.words = np.array(words, dtype=np.int64)
         self.table: Optional[torch.Tensor] = None          # the words on the device, put there by the backend
+
+    def _layout(self, x: torch.Tensor):
+        """(address, bytes from row to row, shape, bytes of an element), of rows that are what they have to be."""
+        shape, strides, item = tuple(x.shape), x.stride(), x.element_size()
+        if x.device != self.device:
+            raise ValueError(f"the tensors of a set of rows lie on one device, got {self.device} and {x.device}")
+        if not shape or 0 in shape:
+            raise ValueError(f"a set of rows takes tensors with rows in them, got shape {shape}")
+        count = 1
+        for n, s in zip(shape[:0:-1], strides[:0:-1]):
+            if n > 1 and s != count:
+                raise ValueError("a row has to be contiguous")
+            count *= n
+        if shape[0] > 1 and strides[0] < count:
+            raise ValueError("rows may not overlap")
+        return x.data_ptr(), strides[0] * item, shape, item
 
     def units(self, tokens: int) -> int:
         """Pieces of at most 16 bytes in what is copied of the largest row where it holds `tokens` tokens (below zero: all)."""

@@ -82,14 +82,13 @@ class LogitRules:
         if biases is not None and len(biases) != rows:
             raise ValueError(f"biases: {len(biases)} values for {rows} rows")
         starts = np.zeros(rows + 1, dtype=np.int64)
-        tokens: List[int] = []
-        values: List[float] = []
+        if biases is not None:
+            np.cumsum([len(row) if row else 0 for row in biases], out=starts[1:])
+        ids, add = np.empty(starts[-1], dtype=np.int64), np.empty(starts[-1], dtype=np.float64)
         for i, row in enumerate(biases or ()):
             if row:
-                tokens.extend(row.keys())
-                values.extend(row.values())
-            starts[i + 1] = len(tokens)
-        ids, add = np.array(tokens, dtype=np.int64), np.array(values, dtype=np.float64)
+                a, b = starts[i], starts[i + 1]
+                ids[a:b], add[a:b] = np.fromiter(row.keys(), np.int64, b - a), np.fromiter(row.values(), np.float64, b - a)
         if ids.size:
             if ids.min() < 0 or ids.max() >= vocab:
                 bad = ids.min() if ids.min() < 0 else ids.max()
@@ -130,12 +129,14 @@ def mask_words(vocab: int) -> int:
 def pack_mask(vocab: int, allowed) -> np.ndarray:
     """int32 `[mask_words(vocab)]`, bit t % 32 of word t // 32 set where token t may be chosen. `allowed`: the token ids, or a
     boolean for every token."""
-    a = np.asarray(allowed)
+    a = np.asarray(sorted(allowed) if isinstance(allowed, (set, frozenset)) else allowed)
     if a.dtype == bool:
         if a.shape != (vocab,):
             raise ValueError(f"a mask has a truth value for each of the {vocab} tokens, got shape {a.shape}")
         bits = a
     else:
+        if a.size and a.dtype.kind not in "iu":
+            raise ValueError(f"allowed tokens are whole numbers, or a truth value for each of the {vocab}, got {a.dtype}")
         ids = a.astype(np.int64).reshape(-1)
         if ids.size and (ids.min() < 0 or ids.max() >= vocab):
             bad = ids.min() if ids.min() < 0 else ids.max()
