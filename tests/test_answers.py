@@ -15,10 +15,11 @@ from transformers_neuronx_amd.cache import CacheManager, OutOfPages, OutOfSlots,
 from transformers_neuronx_amd.config import EngineConfig
 from transformers_neuronx_amd.engine import StepEntry
 from transformers_neuronx_amd.engine.engine import LLMEngine
-from transformers_neuronx_amd.engine.factory import runner_from_folder
+from transformers_neuronx_amd.engine.factory import build_runner, runner_from_folder
 from transformers_neuronx_amd.kernels import make_ops
 from transformers_neuronx_amd.parts.base import CacheNeed
 from transformers_neuronx_amd.sampling import Sampler, SamplingParams, Steering
+from transformers_neuronx_amd.weights.loader import TensorDict
 
 BOTH = pytest.mark.parametrize("kernels", ["reference", pytest.param("hip", marks=pytest.mark.gpu)])
 
@@ -620,3 +621,117 @@ def test_rows_reordered_and_sequences_forked(tiny_folders, kernels):
         model.fork_sequence(3, 1)
     with pytest.raises(ValueError):
         model.fork_sequence(0, 0)
+
+
+@BOTH
+@pytest.mark.parametrize("run_ahead, prompts_first", [(True, False), (False, False), (True, True)])
+@pytest.mark.parametrize("design, seed", [("opt", 0), ("opt", 1), ("opt", 2), ("opt", 3)] + [(d, i) for d in CASES for i in range(2)])
+def test_everything_together_in_any_order(tiny_folders, kernels, run_ahead, prompts_first, design, seed):
+    """Families of samples, forks midway, requests taken out, a pool that is too small and changes its size, steered and scored requests
+    among plain ones: each generates what it would alone."""
+    if design == "opt":
+        folder, cfg, _ = tiny_folders["A"]
+        vocab = cfg["vocab_size"]
+
+        def made(**kw):
+            return engine_of(folder, kernels, **kw)
+    else:
+        module, name = CASES[design]
+        cfg = module.config(name)
+        vocab, w = cfg.vocab, module.weights(cfg, 4)
+
+        def made(max_tokens=640, max_num_seqs=8, **kw):
+            ecfg = EngineConfig(dtype="float32", kernels=kernels, device=device_of(kernels), page_size=16, max_tokens=max_tokens,
+                                max_num_seqs=max_num_seqs, **kw)
+            return LLMEngine(build_runner(cfg, TensorDict({k: v.clone() for k, v in w.items()}), ecfg), ecfg)
+    rng = random.Random(seed)
+    engine = made(max_tokens=rng.choice([176, 256, 400]), max_num_seqs=rng.choice([3, 5, 8]), chunk_size=rng.choice([None, 7]),
+                  max_num_batched_tokens=rng.choice([24, 2048]), run_ahead=run_ahead, prompts_first=prompts_first)
+    cache = engine.runner.cache
+    told = {}                     # name -> (prompt, params, tokens it began with)
+    reported = {}
+
+    def rules():
+        return rng.choice([{}, {}, dict(repetition_penalty=1.4), dict(frequency_penalty=0.3, logprobs=2), dict(logprobs=0),
+                           dict(logit_bias={5: 3.0, 9: float("-inf")}), dict(allowed_tokens=sorted(rng.sample(range(vocab), vocab // 3))),
+                           dict(presence_penalty=0.5, allowed_tokens=lambda out: range(len(out) % 7, vocab, 7))])
+    for turn in range(60):
+        what = rng.choice(["add", "step", "step", "step", "fork", "abort", "resize", "compact"])
+        if what == "add" and len(told) < 14:
+            prompt = [rng.randrange(3, vocab) for _ in range(rng.choice([1, 2, 9, 17, 33, 48]))]
+            params = SamplingParams(max_new_tokens=rng.choice([1, 3, 12, 20]), temperature=1.2, top_k=rng.choice([0, 1, 30]), seed=rng.randrange(999),
+                                    ignore_eos=True, **rules())
+            for i, name in enumerate(engine.add_samples(prompt, params, rng.choice([1, 1, 2, 4]), f"n{turn}")):
+                told[name] = prompt, dataclasses.replace(params, seed=params.seed + i), []
+        elif what == "fork" and told:
+            name = rng.choice([n for n in told])
+            if name in engine.requests and len([t for t in engine.requests[name].output if t >= 0]) < told[name][1].max_new_tokens:
+                have = [t for t in engine.requests[name].output if t >= 0]
+                params = dataclasses.replace(told[name][1], seed=rng.randrange(999))
+                told[engine.fork_request(name, params, f"f{turn}")] = told[name][0], params, have
+        elif what == "abort" and len(told) > 3 and rng.random() < 0.4:
+            name = rng.choice([n for n in told])
+            if name in engine.requests:
+                engine.abort_request(name)
+            del told[name]
+            reported.pop(name, None)
+        elif what == "resize" and rng.random() < 0.5:
+            held = max(g.pool.num_pages - g.pool.num_free for g in cache.groups.values())
+            engine.resize_cache(max(held, rng.choice([11, 16, 25])))
+        elif what == "compact":
+            cache.compact()
+        else:
+            for o in engine.step():
+                reported.setdefault(o.req_id, []).append(o.token)
+        cache.check()
+    while engine.has_work:
+        for o in engine.step():
+            reported.setdefault(o.req_id, []).append(o.token)
+    cache.check()
+    assert not cache.requests and all(g.pool.num_free == g.pool.num_pages for g in cache.groups.values())
+    alone = made()
+    for name, (prompt, params, begun) in told.items():
+        q = engine.requests[name]
+        assert q.output == begun + reported[name] and len(q.output) == params.max_new_tokens
+        if params.logprobs is not None:
+            assert len(q.logprobs) == len(q.top_logprobs) == len(q.output)
+        alone.reset()
+        alone.add_request(prompt, params, "x")
+        if begun:
+            # a request that begins with tokens it did not draw itself
+            alone.abort_request("x")
+            alone._add(prompt, params, "x", output=begun)
+        alone.run()
+        assert alone.requests["x"].output == q.output, (name, params)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["A", "C"])
+@pytest.mark.parametrize("graphs", [True, False])
+def test_forked_requests_of_a_bfloat16_engine(tiny_folders_bf16, name, graphs):
+    """Forks of one request, fed the same tokens in one batch, give the same bits, wherever pages move in between."""
+    folder, cfg, _ = tiny_folders_bf16[name]
+    ecfg = EngineConfig(dtype="bfloat16", device="cuda:0", page_size=16, num_pages=60, max_num_seqs=6, use_graphs=graphs)
+    runner = runner_from_folder(folder, ecfg)
+    assert runner.cache.page_pad_bytes == 384
+    prompt = prompts_of(cfg["vocab_size"], [45], 1)[0]
+    runner.step([StepEntry("a", prompt, [])])
+    for i, child in enumerate("bcd"):
+        runner.fork("a", child)
+    names, rng = list("abcd"), random.Random(0)
+    for turn in range(30):
+        token = rng.randrange(3, cfg["vocab_size"])
+        logits = runner.step([StepEntry(n, [token], [0]) for n in names])
+        assert all(torch.equal(logits[0], row) for row in logits[1:]), turn
+        assert torch.isfinite(logits).all()
+        if turn % 5 == 1:
+            runner.finish(names[1])
+            runner.fork(names[3], names[1])
+        elif turn % 5 == 2:
+            runner.reorder(names, [2, 2, 0, 1])
+        elif turn % 5 == 3:
+            runner.cache.compact()
+        elif turn % 10 == 4:
+            runner.resize_cache(30 if turn == 4 else 70)
+        runner.cache.check()
+    assert len(runner.cache.requests["a"].tables["full"]) == 5

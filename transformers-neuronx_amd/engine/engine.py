@@ -89,6 +89,8 @@ class LLMEngine:
             # a stream of the request's own, the same whatever else runs beside it
             params = dataclasses.replace(params, seed=int(self.config.seed) + self._taken)
         req = Request(rid, prompt, params, output=list(output), leader=leader)
+        if params.logprobs is not None:            # (of tokens it begins with nothing is known: 0, and no others)
+            req.logprobs, req.top_logprobs = [0.0] * len(output), [[] for _ in output]
         req.mask = self._mask(req)
         if req.mask is not None and not req.mask.any():
             raise ValueError(f"request {rid!r}: no token is allowed")
@@ -130,12 +132,9 @@ class LLMEngine:
         if params.max_new_tokens <= len(output):
             raise ValueError(f"request {req_id!r} has {len(output)} tokens already, max_new_tokens is {params.max_new_tokens}")
         child = self._add(req.prompt, params, new_id, leader=None if req.finished else req, output=output)
-        if params.logprobs is not None:
-            # of the tokens taken over, what is known of them
+        if params.logprobs is not None and req.params.logprobs is not None:
             q = self.requests[child]
-            known = len(output) if len(req.logprobs) >= len(output) else 0
-            q.logprobs = req.logprobs[:known] + [0.0] * (len(output) - known)
-            q.top_logprobs = req.top_logprobs[:known] + [[] for _ in range(len(output) - known)]
+            q.logprobs, q.top_logprobs = req.logprobs[:len(output)], req.top_logprobs[:len(output)]
         return child
 
     def resize_cache(self, num_pages) -> None:

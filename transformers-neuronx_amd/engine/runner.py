@@ -275,6 +275,7 @@ class ModelRunner:
         if self.model.device.type == "cuda":
             torch.cuda.synchronize(self.model.device)
         self._recorded.clear()
+        self._graph_pool = None          # with the last recording that drew on it the pool is gone
         self._last_ctx = None
         self.cache.resize(num_pages)
         if self.model.device.type == "cuda":
