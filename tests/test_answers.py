@@ -735,3 +735,40 @@ def test_forked_requests_of_a_bfloat16_engine(tiny_folders_bf16, name, graphs):
             runner.resize_cache(30 if turn == 4 else 70)
         runner.cache.check()
     assert len(runner.cache.requests["a"].tables["full"]) == 5
+
+
+@BOTH
+def test_a_search_over_beams(tiny_folders, kernels):
+    """As a program does it with the model's own calls: the likeliest continuations of every beam, the best of them all kept, the cache
+    reordered. Against the same search over whole sequences without a cache, in 64 bits."""
+    import plain_opt
+    folder, cfg, weights = tiny_folders["A"]
+    prompt, beams, new = prompts_of(cfg["vocab_size"], [18], 12)[0], 3, 12
+    want = [(0.0, [])]
+    for _ in range(new):
+        every = []
+        for score, tail in want:
+            lp = torch.log_softmax(plain_opt.forward_logits(weights, cfg, prompt + tail)[-1].double(), -1)
+            every += [(score + float(lp[t]), tail + [int(t)]) for t in torch.topk(lp, beams).indices]
+        want = sorted(every, key=lambda x: -x[0])[:beams]
+    model = model_of(folder, kernels, beams)
+    ops = model.engine.runner.ops
+    logits = model.forward(torch.tensor([prompt]))
+    kept = [(0.0, [])]
+    for step in range(new):
+        rows = len(kept)
+        _, ids, best = ops.log_probs(logits, torch.zeros(rows, dtype=torch.int32, device=logits.device), beams)
+        every = [(kept[b][0] + float(best[b, k]), kept[b][1] + [int(ids[b, k])], b) for b in range(rows) for k in range(beams)]
+        every = sorted(every, key=lambda x: -x[0])[:beams]
+        if rows == 1:
+            for b in range(1, beams):
+                model.engine.runner.fork(("row", 0), ("row", b))
+        else:
+            model.reorder_cache([b for _, _, b in every])
+        kept = [(score, tail) for score, tail, _ in every]
+        if step + 1 < new:
+            logits = model.forward(torch.tensor([[tail[-1]] for _, tail in kept]), cache_ids=[len(prompt) + step])
+        model.engine.runner.cache.check()
+    assert [tail for _, tail in kept] == [tail for _, tail in want]
+    # twelve log-probabilities a beam, each off by what float32 logits of this size are
+    assert all(abs(a - b) < 12 * 3e-5 for (a, _), (b, _) in zip(kept, want))

@@ -534,6 +534,7 @@ class HipOps:
         if self.device.type != "cuda" or not torch.cuda.is_available():
             raise RuntimeError("the HIP kernels need a GPU; none is visible to torch")
         _code(dtype)
+        self._index = self.device.index
         self.compute_units = torch.cuda.get_device_properties(self.device).multi_processor_count
         self._bias_copies = {}
         self._conv_copies = {}
@@ -2896,7 +2897,7 @@ class HipOps:
         if device.type != "cuda":
             raise ValueError(f"{what} must be on the GPU")
         at = torch._C._cuda_getDevice()
-        if device.index != at or self.device.index not in (None, at):
+        if device.index != at or (self._index != at and self._index is not None):
             raise ValueError(f"{what} on {device}, but the current device is cuda:{at} and these kernels work on {self.device}")
 
     def _from_host(self, flat, what):
