@@ -552,6 +552,7 @@ def test_sequences_from_the_entry_point(tiny_folders, kernels):
         assert score[3 * b + chosen] >= score[3 * b:3 * b + 3].max() - 0.05
     greedy = model.sample(ids, 18, top_k=1, repetition_penalty=1e6)
     assert all(len(set(row.tolist()[10:])) == 8 and not set(row.tolist()[10:]) & set(row.tolist()[:10]) for row in greedy)
+    assert torch.equal(model.sample(ids, 7, num_return_sequences=2), ids[[0, 0, 1, 1], :7])        # nothing to generate
     assert (model.sample(ids, 14, top_k=5, allowed_tokens=[40, 41])[:, 10:] // 2 == 20).all()
     for bad in (dict(num_return_sequences=0), dict(num_return_sequences=3, best_of=2)):
         with pytest.raises(ValueError):

@@ -286,11 +286,11 @@ class CausalLMForSampling:
         if prompts.dim() == 1:
             prompts = prompts.unsqueeze(0)
         width = prompts.shape[1]
-        if sequence_length <= width:
-            return prompts[:, :sequence_length].clone()
         made = num_return_sequences if best_of is None else best_of
         if num_return_sequences < 1 or made < num_return_sequences:
             raise ValueError(f"num_return_sequences ({num_return_sequences}) is at least 1 and no more than best_of ({best_of})")
+        if sequence_length <= width:
+            return prompts[:, :sequence_length].repeat_interleave(num_return_sequences, 0)
         if streamer is not None and made > num_return_sequences:
             raise ValueError("which answers are kept is known at their end: best_of has nothing to stream")
         steered = dict(repetition_penalty=repetition_penalty, frequency_penalty=frequency_penalty, presence_penalty=presence_penalty,
