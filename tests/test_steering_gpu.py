@@ -347,6 +347,27 @@ def test_on_another_stream(ops):
     assert torch.equal(t, want)
 
 
+def test_rules_and_rows_made_on_one_stream_and_used_on_another(ops):
+    """What was sent from the host may still be on its way where another stream works by it."""
+    case = random_rules(4, 3001, 500, 30, 0.5, seed=12)
+    logits, _, history, last, masks = _adjust(ops, case)
+    t = torch.randn(6, 5, 64, device="cuda")
+    want = t.clone()
+    want[3] = want[1]
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    torch.cuda._sleep(100_000_000)
+    rules, rows = ops.logit_rules(3001, **case["rules"]), ops.row_set([t])
+    with torch.cuda.stream(side):
+        ops.adjust_logits(logits, rules, history, last, masks)
+        ops.copy_rows(rows, [1], [3])
+        ops.copy_rows(rows, [], [])
+    del rules, rows
+    torch.cuda.synchronize()
+    _check_adjusted(case, logits, history)
+    assert torch.equal(t, want)
+
+
 def test_refusals(ops):
     from transformers_neuronx_amd.kernels.steering import TokenHistory
     x = torch.zeros(2, 40, device="cuda")

@@ -525,6 +525,27 @@ def _want(t: torch.Tensor, name: str, dtype=None, shape=None):
     return t
 
 
+class _Sent:
+    """Words from the host in device memory, which later calls work by, on any stream: one that is not the stream they were sent on waits for
+    them once, since what a kernel would find before they are there is no address and no slot. (A recording begins when all is done
+    that was sent before it.)"""
+
+    __slots__ = ("words", "at", "there", "streams")
+
+    def __init__(self, words: torch.Tensor):
+        self.words, self.at, self.there, self.streams = words, words.data_ptr(), torch.cuda.Event(), {_stream()}
+        self.there.record()
+
+    def reached(self, stream: int) -> int:
+        """Their address, for a launch on `stream`, the current one."""
+        if stream not in self.streams and not torch.cuda.is_current_stream_capturing():
+            here = torch.cuda.current_stream()
+            here.wait_event(self.there)
+            self.words.record_stream(here)
+            self.streams.add(stream)
+        return self.at
+
+
 class HipOps:
     name = "hip"
 
@@ -2905,7 +2926,7 @@ class HipOps:
         pinned memory holds by then."""
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError(f"{what} takes lists from the host and cannot be recorded into a graph")
-        return self.send_ints(flat)
+        return _Sent(self.send_ints(flat))
 
     def row_set(self, tensors, token_axes=None, targets=None) -> RowSet:
         """See `RowSet`; what `copy_rows` works on."""
@@ -2919,7 +2940,7 @@ class HipOps:
         the tensor counts tokens, or whole (`tokens` None, or a tensor without a token axis). What lies behind them stays as it
         was. The rows are lists on the host; a source may be named several times, a target once and not as a source too."""
         pairs = rows.pairs(sources, targets, tokens)
-        if rows.table is None:
+        if not isinstance(rows.table, _Sent):
             raise ValueError("this set of rows was not made by row_set")
         units = rows.units(max(n for _, n, _ in pairs) if pairs and tokens is not None else -1)
         if not pairs or units == 0:
@@ -2934,8 +2955,9 @@ class HipOps:
             host = (ctypes.c_int * len(words))(*words)
         else:
             dev = self.send_ints(np.array(words, dtype=np.int32))
-        self._call("rows", "tnx_copy_rows", rows.table.data_ptr(), len(rows.tensors), host, len(words), _ptr(dev), len(groups), units,
-                   _stream(), work=lambda: (f"{len(groups)} to {len(pairs)} rows", (len(groups) + len(pairs)) * rows.row_bytes, 0))
+        stream = _stream()
+        self._call("rows", "tnx_copy_rows", rows.table.reached(stream), len(rows.tensors), host, len(words), _ptr(dev), len(groups), units,
+                   stream, work=lambda: (f"{len(groups)} to {len(pairs)} rows", (len(groups) + len(pairs)) * rows.row_bytes, 0))
 
     ROW_WORDS = 256        # of a list of rows that goes along with a launch: 4 a source with its tokens, 1 a target
 
@@ -2975,8 +2997,9 @@ class HipOps:
         flat[:heads.size] = heads.reshape(-1)
         if at:
             flat[room:] = np.concatenate(lists).reshape(-1)
-        dev = self._from_host(flat, "start_history")
-        self._call("steering", "tnx_start_history", _ptr(dev), len(slots), _ptr(dev[room:]), _ptr(history.entries), _ptr(history.used),
+        sent = self._from_host(flat, "start_history")
+        at = sent.at
+        self._call("steering", "tnx_start_history", at, len(slots), at + 4 * room, _ptr(history.entries), _ptr(history.used),
                    _ptr(last), history.slots, history.capacity, _stream())
 
     def logit_rules(self, vocab, rows=None, slots=None, repetition=None, presence=None, frequency=None, biases=None,
@@ -2989,7 +3012,7 @@ class HipOps:
             rows = given[0]
         rules = LogitRules(int(vocab), rows, slots, repetition, presence, frequency, biases, mask_rows)
         if rules.flat.size:
-            rules.placed(self._from_host(rules.flat, "logit_rules"))
+            rules.device_words = self._from_host(rules.flat, "logit_rules")
         return rules
 
     def adjust_logits(self, logits, rules: LogitRules, history: Optional[TokenHistory] = None, last=None, masks=None):
@@ -3003,8 +3026,10 @@ class HipOps:
             return logits
         device = logits.device
         self._on_this_device(device, "logits")
-        if rules.device_words is None or rules.device_words.device != device:
+        if not isinstance(rules.device_words, _Sent) or rules.device_words.words.device != device:
             raise ValueError("these rules were not made by logit_rules, or lie on another device than the logits")
+        stream = _stream()
+        at = rules.device_words.reached(stream)
         entries = used = last_at = masks_at = None
         capacity = 0
         if rules.most_slot >= 0:
@@ -3025,8 +3050,8 @@ class HipOps:
             if rules.most_mask >= masks.shape[0]:
                 raise ValueError(f"mask {rules.most_mask} is outside the {masks.shape[0]} there are")
             masks_at = masks.data_ptr()
-        self._call("steering", "tnx_adjust_logits", logits.data_ptr(), *rules.addresses, entries, used, capacity, last_at, masks_at,
-                   rules.rows, rules.vocab, _stream())
+        self._call("steering", "tnx_adjust_logits", logits.data_ptr(), at, at + rules.tokens_at, at + rules.values_at, entries, used, capacity, last_at, masks_at,
+                   rules.rows, rules.vocab, stream)
         return logits
 
     MOST_TOP = 32         # alternatives that `log_probs` gives at most

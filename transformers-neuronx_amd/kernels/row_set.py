@@ -64,7 +64,7 @@ class RowSet:
         self.row_bytes = sum(w[4] * w[6] for w in words)
         self._shapes = sorted({tuple(w[4:]) for w in words})
         self.words = np.array(words, dtype=np.int64)
-        self.table: Optional[torch.Tensor] = None          # the words on the device, put there by the backend
+        self.table = None                                  # the words on the device, put there by the backend
 
     def _layout(self, x: torch.Tensor):
         """(address, bytes from row to row, shape, bytes of an element), of rows that are what they have to be."""

@@ -107,13 +107,8 @@ class LogitRules:
         flat[n + self.num_biases:] = add.astype(np.float32).view(np.int32)
         self.flat = flat
         self.mask_words = mask_words(vocab)
-        self.device_words: Optional[torch.Tensor] = None      # put there by the backend
-        self.addresses = (None, None, None)                   # of the rules, the biases' tokens and their values there
-
-    def placed(self, words: torch.Tensor) -> None:
-        self.device_words = words
-        at = words.data_ptr()
-        self.addresses = (at, at + 4 * self.rows * self.WORDS, at + 4 * (self.rows * self.WORDS + self.num_biases))
+        self.tokens_at, self.values_at = 4 * n, 4 * (n + self.num_biases)      # bytes before the biases' tokens, and their values
+        self.device_words = None                              # put there by the backend
 
     def pieces(self, words):
         """(rules, bias tokens, bias values) of the words, in whatever memory they lie."""
