@@ -3020,7 +3020,8 @@ class HipOps:
         every token of the history is penalised, x / repetition where x > 0 and x * repetition elsewhere, less
         frequency * times chosen, less presence if it was chosen; the row's biases are added; and tokens whose bit the row's mask
         lacks become -inf, whatever they were. `masks`: int32 `[masks, mask_words(vocab)]`, bit t % 32 of word t // 32 for
-        token t (`pack_mask`). Returns the logits."""
+        token t (`pack_mask`). May be recorded into a graph, which works by the rules' memory: they have to be kept as long as it is
+        replayed. Returns the logits."""
         _want(logits, "logits", torch.float32, (rules.rows, rules.vocab))
         if rules.rows == 0:
             return logits
