@@ -417,3 +417,44 @@ def test_log_probs_sent_to_the_host(ops):
     a = ops.log_probs(logits, tokens, 3)
     with pytest.raises(ValueError):
         ops.send_log_probs(a[0][:4], a[1], a[2])
+
+
+@pytest.mark.parametrize("vocab, copies", [(60, 1), (20001, 1), (700, 6)])
+def test_log_probs_of_maxima_between_ten_millions_and_ten_billions(ops, vocab, copies):
+    """Where one unit of the last place of a logit is more than one, and more than what a power of two can put back."""
+    g = np.random.default_rng(vocab)
+    maxima = np.concatenate([[2000003840, 2007735680, 2.06e9, 2175962880, 3000016896, 3000050432, 5000029696, 5.58e9, 5661881856, 10000146432, 10618571776],
+                             10.0 ** g.uniform(7, 13, 50)])
+    maxima = np.tile(np.concatenate([maxima, -maxima]).astype(np.float32), copies)          # (and as many rows as smaller blocks take)
+    x = g.normal(0, 3, (len(maxima), vocab)).astype(np.float32)
+    below = np.nextafter(maxima, np.float32(-np.inf))
+    low = maxima < 0
+    x[low] = maxima[low, None] * (1 + np.abs(x[low]))
+    at, near, tie = g.permuted(np.tile(np.arange(vocab), (len(maxima), 1)), axis=1)[:, :3].T
+    rows = np.arange(len(maxima))
+    x[rows, near], x[rows, at] = below, maxima
+    x[rows[::3], tie[::3]] = maxima[::3]
+    tokens = np.where(rows % 2, at, near).astype(np.int32)
+    got = ops.log_probs(torch.from_numpy(x).cuda(), torch.from_numpy(tokens).cuda(), 3)
+    want, ids, best = log_probs_in_64(x, tokens, 3)
+    # a thread adds a 512th of the row term by term, the threads' sums meet in ten additions; the rest are the roundings of the power and
+    # its argument (at most 8 and a half where it is not one by one), of the logarithm and of the two differences
+    steps = 20 + vocab / 512
+    for a, b in ((got[0], want), (got[2], best)):
+        a = a.cpu().numpy().astype(np.float64)
+        off = ~np.isfinite(a).reshape(len(maxima), -1).all(1)
+        assert not off.any(), maxima[off][:20]
+        assert (np.abs(a - b) <= steps * 2.0 ** -24 * (1 + np.abs(b))).all()
+    assert np.array_equal(got[1].cpu().numpy(), ids)
+
+
+def test_log_probs_of_a_long_row_are_off_by_a_few_roundings(ops):
+    """16 logits of a round are added up by two chains of eight, rounds one by one, threads' sums in at most ten additions."""
+    for rows, vocab in ((3, 50272), (600, 50272), (2, 200003), (1, 5000)):
+        x = torch.randn(rows, vocab, generator=torch.Generator(device="cuda").manual_seed(rows), device="cuda") * 2
+        tokens = torch.arange(rows, device="cuda", dtype=torch.int32)
+        want = x.double()[torch.arange(rows), :rows].diagonal() - torch.logsumexp(x.double(), 1)
+        got = ops.log_probs(x, tokens)[0].double()
+        # and eight more for the powers, their arguments, the logarithm and the differences
+        steps = 8 + -(-vocab // (16 * 512)) + 10 + 8
+        assert ((got - want).abs() <= steps * 2.0 ** -24 * (1 + want.abs())).all()

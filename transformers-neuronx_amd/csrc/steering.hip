@@ -202,8 +202,9 @@ struct PowersBelow {
   __device__ __forceinline__ float operator()(float x) const { return __builtin_amdgcn_exp2f(fmaf(x, LOG2E_HI, shift)); }
   __device__ __forceinline__ float back() const { return __builtin_amdgcn_exp2f(lost); }
 };
-// Beyond this many powers overflow on the way; rows with such a maximum are summed again with care.
-#define SCORE_FAR 1e30f
+// `lost` is up to half a unit in the last place of r log2(e): 8 where |r| is just below this, from about 1.4e9 on beyond what the
+// hardware's powers hold (2^-126 to 2^128, and less than that is 0). Rows whose maximum lies further out are summed again with care.
+#define SCORE_FAR 1e8f
 
 // A row read four logits at a time from the boundary of 16 bytes at or before it: quad q holds elements 4 q - lead to 4 q - lead + 3;
 // what lies outside the row reads as -inf.
@@ -303,8 +304,8 @@ log_probs_kernel(const float* __restrict__ logits, const int* __restrict__ token
 #pragma unroll
   for (int w = 1; w < WAVES; ++w) m = fmaxf(m, scratch[w]);
   s = block_sum<WAVES>(s * power.back() * exp_of(power.r - m), sums);
-  if (!(s < INFINITY) || !(fabsf(m) < SCORE_FAR)) {
-    // with a NaN somewhere, or a maximum that is far out or none: one by one
+  if (!(s >= 0.5f && s < INFINITY) || !(fabsf(m) < SCORE_FAR)) {
+    // with a NaN somewhere, or a maximum that is far out or none: one by one (the maximum itself is 1 of any sum that is right)
     float exact = 0.f;
     for (int q = tid; q < quads.count; q += THREADS) {
       const f32x4 x = quads(q);
