@@ -773,3 +773,43 @@ def test_a_search_over_beams(tiny_folders, kernels):
     assert [tail for _, tail in kept] == [tail for _, tail in want]
     # twelve log-probabilities a beam, each off by what float32 logits of this size are
     assert all(abs(a - b) < 12 * 3e-5 for (a, _), (b, _) in zip(kept, want))
+
+
+@BOTH
+@pytest.mark.parametrize("how", ["raises", "no token"])
+def test_a_grammar_that_fails_ends_its_request_alone(tiny_folders, kernels, how):
+    folder, cfg, _ = tiny_folders["A"]
+    vocab = cfg["vocab_size"]
+    prompts = prompts_of(vocab, [9, 12, 7], 2)
+
+    def fails(output):
+        if len(output) == 4 and how == "raises":
+            raise KeyError("no rule")
+        return [7, 8, vocab if len(output) == 4 else 9]
+    plain = SamplingParams(max_new_tokens=9, do_sample=False, ignore_eos=True)
+    steered = dataclasses.replace(plain, allowed_tokens=fails, logprobs=0)
+    want = engine_of(folder, kernels).generate(prompts[1:], plain)
+    engine = engine_of(folder, kernels)
+    for name, prompt, params in (("a", prompts[1], plain), ("b", prompts[0], steered), ("c", prompts[2], plain)):
+        engine.add_request(prompt, params, name)
+    reported, ends = {}, {}
+    while engine.has_work:
+        for o in engine.step():
+            reported.setdefault(o.req_id, []).append(o.token)
+            if o.finished:
+                ends[o.req_id] = o.finish_reason
+    assert [reported["a"], reported["c"]] == want and ends == {"a": "length", "b": "error", "c": "length"}
+    b = engine.requests["b"]
+    assert reported["b"] == b.output and len(b.output) == len(b.logprobs) == 4 and set(b.output) <= {7, 8, 9}
+    assert isinstance(b.error, KeyError if how == "raises" else ValueError) and engine.requests["a"].error is None
+    engine.runner.cache.check()
+    assert not engine.runner.cache.requests
+    # calls that give whole answers raise it, and nothing is left behind
+    engine = engine_of(folder, kernels)
+    for kw in (dict(), dict(samples=2), dict(samples=1, best_of=3)):
+        with pytest.raises(type(b.error)):
+            engine.generate(prompts[:2], [steered, plain], **kw)
+        assert not engine.has_work and not engine.requests and not engine.runner.cache.requests
+    with pytest.raises(type(b.error)):
+        model_of(folder, kernels).sample(torch.tensor(prompts[:1]), 20, allowed_tokens=fails)
+    assert engine.generate(prompts[1:], plain) == want

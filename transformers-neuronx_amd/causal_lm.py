@@ -340,6 +340,7 @@ class CausalLMForSampling:
                 column += 1
         if streamer is not None:
             streamer.end()
+        engine.raise_errors([engine.requests[i] for i in ids])
         if made > num_return_sequences:
             families = [sorted(ids[b * made:(b + 1) * made], key=lambda i: -engine.requests[i].cumulative_logprob)[:num_return_sequences]
                         for b in range(len(rows))]

@@ -233,9 +233,14 @@ class LLMEngine:
         for r, t in zip(step.runs, kept):
             q = r.request
             if t is not None and not q.finished and q.mask is not None and (q.params.follows_grammar or q.params.no_repeat_ngram_size):
-                q.mask = self._mask(q)
-                if not q.mask.any():
-                    self.scheduler.end(q, "grammar")
+                try:
+                    q.mask = self._mask(q)
+                except Exception as error:         # the caller's function is at fault: this request ends, the others' tokens are theirs
+                    q.error = error
+                    self.scheduler.end(q, "error")
+                else:
+                    if not q.mask.any():
+                        self.scheduler.end(q, "grammar")
         self.scheduler.finished.clear()        # the engine reports ends through `StepOutput`; nothing piles up
         if self.record_timings:
             self.runner.ops.synchronize()
@@ -330,13 +335,19 @@ class LLMEngine:
             plist = [sp if sp.logprobs is not None else dataclasses.replace(sp, logprobs=0) for sp in plist]
         families = [self.add_samples(p, sp, made) if made > 1 else [self.add_request(p, sp)] for p, sp in zip(prompts, plist)]
         self.run()
-        out = []
-        for names in families:
-            family = [self.pop_request(name) for name in names]
-            if made > samples:
-                family = sorted(family, key=lambda q: -q.cumulative_logprob)[:samples]     # (of equal ones the earlier)
-            out.append(family)
+        out = [[self.pop_request(name) for name in names] for names in families]
+        for family in out:
+            self.raise_errors(family)
+        if made > samples:
+            out = [sorted(family, key=lambda q: -q.cumulative_logprob)[:samples] for family in out]     # (of equal ones the earlier)
         return out
+
+    @staticmethod
+    def raise_errors(requests: Sequence[Request]) -> None:
+        """What the function of one of these requests raised (`Request.error`), for callers that see no `StepOutput`."""
+        for q in requests:
+            if q.error is not None:
+                raise q.error
 
     def abort_request(self, req_id: Hashable) -> Request:
         """Stop a request whose caller has gone, between two calls of `step()`: its pages and its slot are

@@ -64,6 +64,7 @@ class Request:
     # of every token of the output, where the request asks for them
     logprobs: List[float] = field(default_factory=list)
     top_logprobs: List[list] = field(default_factory=list)
+    error: Optional[Exception] = field(default=None, repr=False)   # what `allowed_tokens` raised, of a request that ended for it
 
     @property
     def tokens(self) -> List[int]:

@@ -38,7 +38,9 @@ class SamplingParams:
     allowed_tokens  the tokens that may be chosen: their ids, or a truth value for every token of the vocabulary; all
                  others are barred, whatever their biases. A function of the list of tokens generated so far that gives
                  either steers the request through a grammar; the request ends, with the reason "grammar", where
-                 nothing is allowed after a token (a request for which nothing is allowed to begin with is refused)
+                 nothing is allowed after a token (a request for which nothing is allowed to begin with is refused). Where
+                 the function raises, or names what is no token, its request alone ends, with the reason "error"
+                 and the exception as its `error`; calls that give whole answers raise it once all have ended
     logprobs     an integer: each token is reported with its log-probability and with those of this many tokens of the
                  largest logits (0: its own alone). They are those of the logits that the token was chosen from, with
                  penalties, biases and bars, before temperature, top-k and top-p; None: not reported
