@@ -813,3 +813,40 @@ def test_a_grammar_that_fails_ends_its_request_alone(tiny_folders, kernels, how)
     with pytest.raises(type(b.error)):
         model_of(folder, kernels).sample(torch.tensor(prompts[:1]), 20, allowed_tokens=fails)
     assert engine.generate(prompts[1:], plain) == want
+
+
+@BOTH
+def test_forks_without_params_draw_from_streams_of_their_own(tiny_folders, kernels):
+    folder, cfg, _ = tiny_folders["A"]
+    prompt = prompts_of(cfg["vocab_size"], [11], 4)[0]
+    params = SamplingParams(max_new_tokens=20, temperature=1.5, seed=3, ignore_eos=True)
+    engine = engine_of(folder, kernels, max_num_seqs=16, max_tokens=2048)
+    names = engine.add_samples(prompt, params, 3, "a")
+    for _ in range(5):
+        engine.step()
+    have = [t for t in engine.requests["a"].output if t >= 0]
+    forked = [engine.fork_request("a"), engine.fork_request("a"), engine.fork_request(names[1])]
+    forked += [engine.fork_request(forked[0]), engine.fork_request("a", dataclasses.replace(params, temperature=1.4, seed=50))]
+    forked += [engine.fork_request(forked[-1]), engine.fork_request(forked[-1])]
+    engine.run()
+    forked.append(engine.fork_request(names[0], dataclasses.replace(params, max_new_tokens=24)))        # of one that has ended
+    forked.append(engine.fork_request(forked[-1]))
+    engine.run()
+    every = [engine.requests[n] for n in names + forked]
+    assert engine.requests[forked[-2]].params.seed == 3               # (as it was told)
+    seeds = [q.params.seed for q in every if q.req_id != forked[-2]]
+    assert len(set(seeds)) == len(seeds) == 11 and seeds[:3] == [3, 4, 5]
+    assert all(engine.requests[n].output[:len(have)] == have for n in forked[:2])
+    outs = [tuple(q.output) for q in every[:-2]]
+    assert len(set(outs)) == len(outs)
+    # a stream is the same whenever the same is asked for, and a seed of 64 bits has forks too
+    again = engine_of(folder, kernels, max_num_seqs=16, max_tokens=2048)
+    again.add_samples(prompt, params, 3, "a")
+    for _ in range(5):
+        again.step()
+    first = again.fork_request("a")
+    again.add_request(prompt, dataclasses.replace(params, seed=2 ** 63 - 1), "far")
+    far = [again.fork_request("far") for _ in range(2)]
+    again.run()
+    assert again.requests[first].output == engine.requests[forked[0]].output
+    assert len({tuple(again.requests[n].output) for n in ["far"] + far}) == 3

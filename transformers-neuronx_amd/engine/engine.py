@@ -17,7 +17,7 @@ from ..kernels.steering import pack_mask
 from ..sampling.sampler import Sampler, Steering, banned_ngram_tokens
 from .batch import StepEntry
 from .runner import ModelRunner
-from .scheduler import PENDING, Request, ScheduledRun, Scheduler
+from .scheduler import PENDING, Family, Request, ScheduledRun, Scheduler
 
 
 @dataclass
@@ -75,7 +75,7 @@ class LLMEngine:
         return self._add(prompt, params, req_id)
 
     def _add(self, prompt: Sequence[int], params: SamplingParams, req_id: Optional[Hashable], leader: Optional[Request] = None,
-             output: Sequence[int] = ()):
+             output: Sequence[int] = (), family: Optional[Family] = None):
         rid = req_id if req_id is not None else next(self._ids)
         if rid in self.requests and not self.requests[rid].finished:
             raise ValueError(f"request {rid!r} is already live")
@@ -88,7 +88,7 @@ class LLMEngine:
         if params.seed is None:
             # a stream of the request's own, the same whatever else runs beside it
             params = dataclasses.replace(params, seed=int(self.config.seed) + self._taken)
-        req = Request(rid, prompt, params, output=list(output), leader=leader)
+        req = Request(rid, prompt, params, output=list(output), leader=leader, family=family or Family(int(params.seed)))
         if params.logprobs is not None:            # (of tokens it begins with nothing is known: 0, and no others)
             req.logprobs, req.top_logprobs = [0.0] * len(output), [[] for _ in output]
         req.mask = self._mask(req)
@@ -123,15 +123,16 @@ class LLMEngine:
 
     def fork_request(self, req_id: Hashable, params: Optional[SamplingParams] = None, new_id: Optional[Hashable] = None) -> Hashable:
         """Another request that goes on from where `req_id` stands, with its prompt and the tokens that have been reported of it, by
-        `params` (its own with the seed that follows, if not given; `max_new_tokens` counts the tokens taken over too). It shares the
-        pages of the tokens it has in common while `req_id` runs; where it cannot, they are computed again. Its name is returned."""
+        `params` (its own with a random stream that no other of them has, if not given; `max_new_tokens` counts the tokens taken over
+        too). It shares the pages of the tokens it has in common while `req_id` runs; where it cannot, they are computed again. Its name
+        is returned."""
         req = self.requests[req_id]
         output = req.output[:req.output.index(PENDING)] if PENDING in req.output else list(req.output)
         if params is None:
-            params = dataclasses.replace(req.params, seed=(req.params.seed or 0) + 1)
+            params = dataclasses.replace(req.params, seed=req.family.next_seed())
         if params.max_new_tokens <= len(output):
             raise ValueError(f"request {req_id!r} has {len(output)} tokens already, max_new_tokens is {params.max_new_tokens}")
-        child = self._add(req.prompt, params, new_id, leader=None if req.finished else req, output=output)
+        child = self._add(req.prompt, params, new_id, leader=None if req.finished else req, output=output, family=req.family)
         if params.logprobs is not None and req.params.logprobs is not None:
             q = self.requests[child]
             q.logprobs, q.top_logprobs = req.logprobs[:len(output)], req.top_logprobs[:len(output)]

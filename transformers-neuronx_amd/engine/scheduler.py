@@ -41,6 +41,18 @@ from ..sampling.params import SamplingParams
 PENDING = -1              # stands in `Request.output` for a token that is drawn but not read yet
 
 
+@dataclass
+class Family:
+    """A request and all that were forked from it, and from those: no two of them draw from one random stream unless they are told to."""
+    seed: int
+    forks: int = 0
+
+    def next_seed(self) -> int:
+        """A seed that no other of the family has, nor the samples of a prompt beside it, whose seeds follow one another."""
+        self.forks += 1
+        return (self.seed + (self.forks << 40) + 2 ** 63) % 2 ** 64 - 2 ** 63
+
+
 @dataclass(eq=False)      # a request is itself: lists of requests are searched by identity
 class Request:
     req_id: Hashable
@@ -59,6 +71,7 @@ class Request:
     leader: Optional["Request"] = field(default=None, repr=False)
     shared: int = 0
     followers: List["Request"] = field(default_factory=list, repr=False)      # that wait for this one
+    family: Optional[Family] = field(default=None, repr=False)
     mask: Optional[object] = field(default=None, repr=False)   # the tokens that may be chosen next (`pack_mask`); None: all
     history_of: Optional[tuple] = None      # the (slot, preemptions) under which the device keeps its history
     # of every token of the output, where the request asks for them
