@@ -850,3 +850,35 @@ def test_forks_without_params_draw_from_streams_of_their_own(tiny_folders, kerne
     again.run()
     assert again.requests[first].output == engine.requests[forked[0]].output
     assert len({tuple(again.requests[n].output) for n in ["far"] + far}) == 3
+
+
+@BOTH
+@pytest.mark.parametrize("run_ahead", [True, False])
+def test_prompts_that_waited_for_pages_go_first_once_there_are_some(tiny_folders, kernels, run_ahead):
+    """`prompts_first` holds again when a pool that was too small has been made larger."""
+    folder, cfg, _ = tiny_folders["A"]
+    engine = engine_of(folder, kernels, max_tokens=64, prompts_first=True, run_ahead=run_ahead)
+    for i, p in enumerate(prompts_of(cfg["vocab_size"], [20, 30, 18], 6)):
+        engine.add_request(p, SamplingParams(max_new_tokens=8, do_sample=False, ignore_eos=True), i)
+    seen = []
+    step = engine.runner.step
+    engine.runner.step = lambda entries, **kw: (seen.append([(e.req, len(e.tokens)) for e in entries]), step(entries, **kw))[1]
+    for _ in range(3):
+        engine.step()
+    assert seen == [[(0, 20), (1, 30)], [(0, 1), (1, 1)], [(0, 1), (1, 1)]] and engine.scheduler.waiting[0].req_id == 2
+    engine.resize_cache(40)
+    engine.step()
+    assert seen[3] == [(2, 18)]
+    engine.run()
+    want = engine_of(folder, kernels).generate(prompts_of(cfg["vocab_size"], [20, 30, 18], 6),
+                                               SamplingParams(max_new_tokens=8, do_sample=False, ignore_eos=True))
+    assert [engine.requests[i].output for i in range(3)] == want
+    # a pool that is too small still lets the requests that can end go on
+    engine = engine_of(folder, kernels, max_tokens=64, prompts_first=True, run_ahead=run_ahead)
+    for i, p in enumerate(prompts_of(cfg["vocab_size"], [20, 30, 18], 6)):
+        engine.add_request(p, SamplingParams(max_new_tokens=8, do_sample=False, ignore_eos=True), i)
+    for size in (4, 5, 4, 4, 5):
+        engine.step()
+        engine.resize_cache(size)
+    engine.run()
+    assert [engine.requests[i].output for i in range(3)] == want

@@ -141,6 +141,7 @@ class LLMEngine:
     def resize_cache(self, num_pages) -> None:
         """Another number of cache pages, between two steps; live requests keep theirs (`ModelRunner.resize_cache`)."""
         self.runner.resize_cache(num_pages)
+        self.scheduler.pool_resized()
 
     def _mask(self, req: Request):
         """The tokens that may come next, where the request says which: those it allows but for those barred otherwise."""

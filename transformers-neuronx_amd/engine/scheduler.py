@@ -135,7 +135,7 @@ class Scheduler:
         self.finished: List[Request] = []
         self._arrivals = 0
         self.num_preemptions = 0
-        self._short = False      # pages have run out and no request has ended since
+        self._short = False      # pages have run out and none have come back since: no request has ended, the pool is what it was
 
     # ---------------------------------------------------------------- arrivals
 
@@ -168,6 +168,10 @@ class Scheduler:
         self.running.clear()
         self.finished.clear()
         self.num_preemptions = 0
+        self._short = False
+
+    def pool_resized(self) -> None:
+        """The page pool is another: what waited for pages is tried again."""
         self._short = False
 
     # ---------------------------------------------------------------- requests that go on from others
@@ -262,7 +266,7 @@ class Scheduler:
         blocked = False                       # pages ran out: admit nothing new this step
         # With `prompts_first` decoding requests wait while a prompt is waiting or under way, but only as
         # long as prompts can get on: once pages have run out (`_short`, until a request ends and frees
-        # some) the decoding requests go first again, since only they can end and free pages; and a step
+        # some or the pool is resized) the decoding requests go first again, since only they can end and free pages; and a step
         # in which no prompt could be planned (no slot, no page) is given to them too.
         hold = (self.prompts_first and not self._short
                 and (bool(self.waiting) or any(not r.decoding for r in self.running)))
