@@ -882,3 +882,56 @@ def test_prompts_that_waited_for_pages_go_first_once_there_are_some(tiny_folders
         engine.resize_cache(size)
     engine.run()
     assert [engine.requests[i].output for i in range(3)] == want
+
+
+def everything_of(m):
+    """What the tables say and what the tensors hold of every request, as values to compare."""
+    out = {}
+    for req, r in m.requests.items():
+        out[req] = (r.slot, r.num_tokens, {g: list(t) for g, t in r.tables.items()},
+                    [t[[p for p in r.tables[lc.group] if p >= 0]].tolist() for lc in m.caches.values() if lc.group for t in lc.pages.values()],
+                    [t[r.slot].tolist() for lc in m.caches.values() for t in lc.state.values()])
+    return out, sorted(m.slots._free), {n: sorted(g.pool._free) for n, g in m.groups.items()}
+
+
+@BOTH
+@pytest.mark.parametrize("state", [False, True])
+def test_a_reorder_that_fails_changes_nothing(kernels, state, monkeypatch):
+    from types import SimpleNamespace
+    from transformers_neuronx_amd.engine.runner import ModelRunner
+    m = manager(kernels, state=state, num_pages=30, max_seqs=5)
+    runner = SimpleNamespace(cache=m, raise_if_lost=lambda: None)
+    names, held = list("abcd"), {}
+    for i, name in enumerate(names):
+        m.add_request(name)
+        held[name] = [100 * i + k for k in range(1, 46)]
+        m.grow(name, 45)
+        fill(m, name, 0, held[name])
+        m.advance(name, 45)
+        if state:
+            for t in m.caches[3].state.values():
+                t[m.slot_of(name)] = i + 1.0
+    m.fork("a", "e")
+    m.free_request("e")
+    before = everything_of(m)
+    copy, calls = m.ops.copy_rows, []
+    for fails_at in range(1, 3 + state):                     # of the pages of two groups, and the slots
+        calls.clear()
+
+        def fails(*a):
+            calls.append(a)
+            if len(calls) == fails_at:
+                raise MemoryError
+            return copy(*a)
+        monkeypatch.setattr(m.ops, "copy_rows", fails)
+        with pytest.raises(MemoryError):
+            ModelRunner.reorder(runner, names, [2, 2, 0, 2])
+        monkeypatch.setattr(m.ops, "copy_rows", copy)
+        m.check()
+        assert everything_of(m) == before, fails_at
+    ModelRunner.reorder(runner, names, [2, 2, 0, 2])
+    m.check()
+    for name, p in zip(names, [2, 2, 0, 2]):
+        holds(m, name, held[names[p]])
+        assert not state or all((t[m.slot_of(name)] == p + 1).all() for t in m.caches[3].state.values())
+    assert sorted(m.requests) == names

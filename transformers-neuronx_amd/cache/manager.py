@@ -285,23 +285,112 @@ class CacheManager:
         mine = self.requests[child] = RequestPages(slot, n, {name: [] for name in self.groups})
         try:
             for g in self.groups.values():
-                first, theirs, table = self._first_block(g, n), r.tables[g.name], mine.tables[g.name]
-                shared = theirs[first:full]
-                g.pool.share(shared, child)
-                table += [-1] * min(first, full) + shared
+                theirs, table = r.tables[g.name], mine.tables[g.name]
+                table += self._share(g, r, n, child)
                 if rest:
                     table += g.pool.allocate(1, child)
-                    if self.allocated:
-                        rows = self._rows(g.name, True)
-                        self.ops.copy_rows(rows, [theirs[full]], [table[-1]], [rest] if rows.places is not None else None)
-            if self.allocated and self.has_state:
-                if self._state_rows is None:
-                    self._state_rows = self.ops.row_set(self._state_tensors())
-                self.ops.copy_rows(self._state_rows, [r.slot], [slot])
+                    self._copy_pages(g, [theirs[full]], [table[-1]], [rest])
+            self._copy_state([r.slot], [slot])
         except Exception:
             self.free_request(child)
             raise
         return slot
+
+    def _share(self, g: PageGroup, r: RequestPages, num_tokens: int, child: Hashable) -> List[int]:
+        """The table of a request that holds the full pages of these tokens too."""
+        first, full = self._first_block(g, num_tokens), num_tokens // self.page_size
+        shared = r.tables[g.name][first:full]
+        g.pool.share(shared, child)
+        return [-1] * min(first, full) + shared
+
+    def _copy_pages(self, g: PageGroup, sources: List[int], targets: List[int], tokens: List[int]) -> None:
+        if self.allocated and targets:
+            rows = self._rows(g.name, True)
+            self.ops.copy_rows(rows, sources, targets, tokens if rows.places is not None else None)
+
+    def _copy_state(self, sources: List[int], targets: List[int]) -> None:
+        if self.allocated and self.has_state and targets:
+            if self._state_rows is None:
+                self._state_rows = self.ops.row_set(self._state_tensors())
+            self.ops.copy_rows(self._state_rows, sources, targets)
+
+    def reorder(self, names: List[Hashable], parents: List[int]) -> None:
+        """Request `names[i]` becomes what `names[parents[i]]` holds now: one that nobody goes on from is over, one that several go on
+        from is forked for all but one of them. All of it or nothing: what is refused is refused first; then pages and slots are set
+        aside, free ones before those of requests that are over; then they are copied to, one launch a group; the tables and names
+        change last, and nothing of that can fail. (Where a launch fails behind another that has run, pages of requests that would have
+        been over may have been written.)"""
+        parents = [int(p) for p in parents]
+        if len(parents) != len(names) or len(set(names)) != len(names):
+            raise ValueError(f"{len(names)} requests, of unlike names, and a parent for each, got {len(parents)}")
+        if any(not 0 <= p < len(names) for p in parents):
+            raise ValueError(f"parents are 0 to {len(names) - 1}, got {parents}")
+        for name in names:
+            if name not in self.requests:
+                raise ValueError(f"request {name!r} is not live")
+        children: Dict[int, List[int]] = {}
+        for i, p in enumerate(parents):
+            children.setdefault(p, []).append(i)
+        over = [name for i, name in enumerate(names) if i not in children]
+        for p, wanted in children.items():           # the first of them takes the parent itself over: it, where it is one of them
+            if p in wanted:
+                wanted.remove(p)
+                wanted.insert(0, p)
+        forks = [(self.requests[names[p]], i) for p, wanted in children.items() for i in wanted[1:]]
+        copied = [(r, i) for r, i in forks if r.num_tokens % self.page_size]
+        if self.allocated and (copied and self.groups or forks and self.has_state):
+            self._copier()
+        held = object()                              # who holds what is set aside
+        aside: Dict[str, List[int]] = {}
+        slots: List[int] = []
+        gone = set(over)
+        try:
+            for g in self.groups.values():
+                free = g.pool.allocate(min(len(copied), g.pool.num_free), held)
+                aside[g.name] = free
+                if len(free) < len(copied):
+                    theirs = dict.fromkeys(p for name in over for p in self.requests[name].tables[g.name]
+                                           if p >= 0 and gone.issuperset(g.pool.holders_of(p)))
+                    more = list(theirs)[:len(copied) - len(free)]
+                    if len(free) + len(more) < len(copied):
+                        raise OutOfPages(f"group {g.name}: {len(copied)} pages wanted, {len(free) + len(theirs)} free")
+                    g.pool.share(more, held)
+                    aside[g.name] = free + more
+            slots += [self.slots.allocate(held) for _ in range(min(len(forks), self.slots.num_free))]
+            taken = over[:len(forks) - len(slots)]
+            into = slots + [self.requests[name].slot for name in taken]
+            for g in self.groups.values():
+                self._copy_pages(g, [r.tables[g.name][r.num_tokens // self.page_size] for r, _ in copied], aside[g.name],
+                                 [r.num_tokens % self.page_size for r, _ in copied])
+            self._copy_state([r.slot for r, _ in forks], into)
+        except Exception:
+            for name, pages in aside.items():
+                self.groups[name].pool.free(pages, held)
+            for s in slots:
+                self.slots.free(s, held)
+            raise
+        marks = [object() for _ in names]            # names of nobody, until all have theirs
+        for name in taken:
+            self.slots.rename(self.requests[name].slot, name, held)
+        for name in over:
+            r = self.requests.pop(name)
+            for g in self.groups.values():
+                g.pool.free([p for p in r.tables[g.name] if p >= 0], name)
+            if name not in taken:
+                self.slots.free(r.slot, name)
+        for slot, (r, i) in zip(into, forks):
+            mine = self.requests[marks[i]] = RequestPages(slot, r.num_tokens, {})
+            self.slots.rename(slot, held, marks[i])
+            for g in self.groups.values():
+                table = mine.tables[g.name] = self._share(g, r, r.num_tokens, marks[i])
+                if r.num_tokens % self.page_size:
+                    page = aside[g.name].pop(0)
+                    g.pool.rename([page], held, marks[i])
+                    table.append(page)
+        for p, wanted in children.items():
+            self.rename(names[p], marks[wanted[0]])
+        for mark, name in zip(marks, names):
+            self.rename(mark, name)
 
     def rename(self, req: Hashable, name: Hashable) -> None:
         """The request goes by another name from now on."""

@@ -17,7 +17,6 @@ import torch
 import numpy as np
 
 from ..cache.manager import CacheManager
-from ..cache.pages import OutOfPages
 from .. import debug
 from ..kernels import LostStep
 from .batch import PackedStep, StepContext, StepEntry, context_from, pack_step
@@ -239,34 +238,10 @@ class ModelRunner:
 
     def reorder(self, names: List[Hashable], parents: List[int]) -> None:
         """Request `names[i]` becomes what `names[parents[i]]` holds now, as a search over beams wants it after each choice: one that
-        nobody goes on from is over, one that several go on from is forked, and no page moves for one that a single other takes over."""
-        if len(parents) != len(names) or len(set(names)) != len(names):
-            raise ValueError(f"{len(names)} requests, of unlike names, and a parent for each, got {len(parents)}")
-        if any(not 0 <= int(p) < len(names) for p in parents):
-            raise ValueError(f"parents are 0 to {len(names) - 1}, got {list(parents)}")
-        for name in names:
-            if not self.cache.has(name):
-                raise ValueError(f"request {name!r} is not live")
+        nobody goes on from is over, one that several go on from is forked, and no page moves for one that a single other takes over: see
+        `CacheManager.reorder`."""
         self.raise_if_lost()
-        children: Dict[int, List[int]] = {}
-        for i, p in enumerate(parents):
-            children.setdefault(int(p), []).append(i)
-        short = {g: sum(len(c) - 1 for p, c in children.items() if self.cache.num_tokens(names[p]) % self.cache.page_size)
-                 for g in self.cache.groups}
-        over = {name for i, name in enumerate(names) if i not in children}
-        for g, n in short.items():
-            freed = len({p for r in over for p in self.cache.requests[r].tables[g]
-                         if p >= 0 and over.issuperset(self.cache.groups[g].pool.holders_of(p))})
-            if n > self.cache.groups[g].pool.num_free + freed:
-                raise OutOfPages(f"group {g}: {n} pages wanted, {self.cache.groups[g].pool.num_free} free")
-        for name in over:
-            self.cache.free_request(name)
-        for p, wanted in children.items():
-            for i in wanted[1:]:
-                self.cache.fork(names[p], ("reordered", i))
-            self.cache.rename(names[p], ("reordered", wanted[0]))
-        for i, name in enumerate(names):
-            self.cache.rename(("reordered", i), name)
+        self.cache.reorder(names, parents)
 
     def resize_cache(self, num_pages) -> None:
         """Pools of another number of pages, with what live requests hold carried over (`CacheManager.resize`). Recorded steps hold the
