@@ -935,3 +935,43 @@ def test_a_reorder_that_fails_changes_nothing(kernels, state, monkeypatch):
         holds(m, name, held[names[p]])
         assert not state or all((t[m.slot_of(name)] == p + 1).all() for t in m.caches[3].state.values())
     assert sorted(m.requests) == names
+
+
+@BOTH
+def test_a_search_over_beams_by_the_calls_of_the_model_alone(tiny_folders, kernels):
+    """From one row of a prompt: `forward`, `reorder_cache`, `forward` and so on. Against whole sequences without a cache."""
+    import plain_opt
+    folder, cfg, weights = tiny_folders["A"]
+    prompt, beams, new = prompts_of(cfg["vocab_size"], [21], 14)[0], 4, 9
+    want = [(0.0, [])]
+    for _ in range(new):
+        every = []
+        for score, tail in want:
+            lp = torch.log_softmax(plain_opt.forward_logits(weights, cfg, prompt + tail)[-1].double(), -1)
+            every += [(score + float(lp[t]), tail + [int(t)]) for t in torch.topk(lp, beams).indices]
+        want = sorted(every, key=lambda x: -x[0])[:beams]
+    model = model_of(folder, kernels, beams)
+    logits, kept = model.forward(torch.tensor([prompt])), [(0.0, [])]
+    for step in range(new):
+        lp = torch.log_softmax(logits.double(), -1).cpu()
+        every = sorted(((kept[b][0] + float(lp[b, t]), kept[b][1] + [int(t)], b) for b in range(len(kept))
+                        for t in torch.topk(lp[b], beams).indices), key=lambda x: -x[0])[:beams]
+        model.reorder_cache(torch.tensor([b for _, _, b in every]))
+        kept = [(score, tail) for score, tail, _ in every]
+        if step + 1 < new:
+            logits = model.forward(torch.tensor([[tail[-1]] for _, tail in kept]), cache_ids=[len(prompt) + step])
+    assert [tail for _, tail in kept] == [tail for _, tail in want]
+    model.engine.runner.cache.check()
+    # no more rows than there are slots, none from a row that is not there, and nothing changes where it is refused
+    before = everything_of(model.engine.runner.cache)
+    for bad, error in (([0] * (beams + 1), OutOfSlots), ([0, 1, 2, 3, 4], ValueError), ([-1, 0, 0, 0], ValueError)):
+        with pytest.raises(error):
+            model.reorder_cache(bad)
+        assert everything_of(model.engine.runner.cache) == before
+    model.forward(torch.tensor([prompt, prompt]))
+    with pytest.raises(ValueError, match="live"):
+        model.reorder_cache([0, 1, 2])
+    model.reorder_cache([1, 0, 0, 1])
+    logits = model.forward(torch.tensor([[5]] * 4), cache_ids=[len(prompt)])
+    assert torch.allclose(logits, logits[:1].expand(4, -1), atol=1e-5 * float(logits.abs().max()))
+    model.engine.runner.cache.check()

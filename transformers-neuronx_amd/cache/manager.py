@@ -316,7 +316,7 @@ class CacheManager:
 
     def reorder(self, names: List[Hashable], parents: List[int]) -> None:
         """Request `names[i]` becomes what `names[parents[i]]` holds now: one that nobody goes on from is over, one that several go on
-        from is forked for all but one of them. All of it or nothing: what is refused is refused first; then pages and slots are set
+        from is forked for all but one of them; a name that nobody has yet is that of a new request. All of it or nothing: what is refused is refused first; then pages and slots are set
         aside, free ones before those of requests that are over; then they are copied to, one launch a group; the tables and names
         change last, and nothing of that can fail. (Where a launch fails behind another that has run, pages of requests that would have
         been over may have been written.)"""
@@ -325,13 +325,13 @@ class CacheManager:
             raise ValueError(f"{len(names)} requests, of unlike names, and a parent for each, got {len(parents)}")
         if any(not 0 <= p < len(names) for p in parents):
             raise ValueError(f"parents are 0 to {len(names) - 1}, got {parents}")
-        for name in names:
-            if name not in self.requests:
-                raise ValueError(f"request {name!r} is not live")
         children: Dict[int, List[int]] = {}
         for i, p in enumerate(parents):
             children.setdefault(p, []).append(i)
-        over = [name for i, name in enumerate(names) if i not in children]
+        for p in children:
+            if names[p] not in self.requests:
+                raise ValueError(f"request {names[p]!r} is not live")
+        over = [name for i, name in enumerate(names) if i not in children and name in self.requests]
         for p, wanted in children.items():           # the first of them takes the parent itself over: it, where it is one of them
             if p in wanted:
                 wanted.remove(p)
@@ -340,6 +340,8 @@ class CacheManager:
         copied = [(r, i) for r, i in forks if r.num_tokens % self.page_size]
         if self.allocated and (copied and self.groups or forks and self.has_state):
             self._copier()
+        if len(forks) > self.slots.num_free + len(over):
+            raise OutOfSlots(f"{len(forks)} request slots wanted, {self.slots.num_free + len(over)} free")
         held = object()                              # who holds what is set aside
         aside: Dict[str, List[int]] = {}
         slots: List[int] = []

@@ -218,7 +218,8 @@ class CausalLMForSampling:
     def reorder_cache(self, beam_idx) -> None:
         """Row b goes on from what row `beam_idx[b]` holds (decoder.py:2262-2319, what a search over beams asks for after each choice):
         rows of a parent share its full pages, and only the page that is not full, and the fixed state, are copied. The rows are those
-        of the last `forward` that began a batch."""
+        of the last `forward` that began a batch; more of them may be asked for, up to the model's batch size: a search begins with
+        one row of the prompt, which becomes as many as it has beams."""
         runner = self._need_engine().runner
         parents = [int(p) for p in torch.as_tensor(beam_idx).flatten()]
         runner.reorder([("row", b) for b in range(len(parents))], parents)
