@@ -975,3 +975,33 @@ def test_a_search_over_beams_by_the_calls_of_the_model_alone(tiny_folders, kerne
     logits = model.forward(torch.tensor([[5]] * 4), cache_ids=[len(prompt)])
     assert torch.allclose(logits, logits[:1].expand(4, -1), atol=1e-5 * float(logits.abs().max()))
     model.engine.runner.cache.check()
+
+
+@BOTH
+def test_a_sequence_is_kept_where_another_cannot_take_its_name(tiny_folders, kernels):
+    from transformers_neuronx_amd import ContinuousBatchingConfig, NeuronConfig
+    folder, cfg, _ = tiny_folders["A"]
+    prompts = prompts_of(cfg["vocab_size"], [19, 16, 13], 3)
+    model = model_of(folder, kernels, 3, num_pages=4, neuron_config=NeuronConfig(continuous_batching=ContinuousBatchingConfig(max_num_seqs=3)))
+
+    def begin(seq, prompt):
+        model.forward(torch.tensor([prompt]), cache_ids=torch.arange(len(prompt)).unsqueeze(0), start_ids=[seq])
+    begin(0, prompts[0])
+    begin(1, prompts[1])
+    cache = model.engine.runner.cache
+    model.fork_sequence(1, 2)                              # a full page needs no copy
+    assert cache.num_tokens(("seq", 2)) == 16
+    model.forward(torch.tensor([[7]]), cache_ids=torch.tensor([[16]]), start_ids=[2])          # the last page
+    before = everything_of(cache)
+    with pytest.raises(OutOfPages):
+        model.fork_sequence(0, 1)                          # a page for the part of a page, and sequence 2 shares the one that 1 holds
+    assert everything_of(cache) == before
+    with pytest.raises(ValueError):
+        model.fork_sequence(5, 1)
+    assert everything_of(cache) == before
+    model.fork_sequence(0, 2)                              # its own page is the one that is needed
+    cache.check()
+    got = model.forward(torch.tensor([[9]]), cache_ids=torch.tensor([[19]]), start_ids=[2])
+    want = model_of(folder, kernels, 3).forward(torch.tensor([prompts[0] + [9]]))
+    assert torch.allclose(got, want, atol=2e-5 * float(want.abs().max()))
+    assert everything_of(cache)[0]["seq", 1] == before[0]["seq", 1]

@@ -229,8 +229,7 @@ class CausalLMForSampling:
         runner = self._need_engine().runner
         if int(seq_id) == int(new_seq_id) or not runner.cache.has(("seq", int(seq_id))):
             raise ValueError(f"sequence {seq_id} holds nothing that sequence {new_seq_id} could go on from")
-        runner.finish(("seq", int(new_seq_id)))
-        runner.fork(("seq", int(seq_id)), ("seq", int(new_seq_id)))
+        runner.reorder([("seq", int(seq_id)), ("seq", int(new_seq_id))], [0, 0])
 
     @torch.no_grad()
     def log_probs(self, input_ids, start_ids=None) -> torch.Tensor:
