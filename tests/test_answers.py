@@ -1005,3 +1005,33 @@ def test_a_sequence_is_kept_where_another_cannot_take_its_name(tiny_folders, ker
     want = model_of(folder, kernels, 3).forward(torch.tensor([prompts[0] + [9]]))
     assert torch.allclose(got, want, atol=2e-5 * float(want.abs().max()))
     assert everything_of(cache)[0]["seq", 1] == before[0]["seq", 1]
+
+
+def test_a_score_of_a_lost_step_is_not_given(tiny_folders):
+    """The last step of a text may be found void when its numbers have reached the host."""
+    from transformers_neuronx_amd.kernels import LostStep
+    folder, cfg, _ = tiny_folders["A"]
+    model = model_of(folder, "reference")
+    runner = model.engine.runner
+    ids = torch.tensor(prompts_of(cfg["vocab_size"], [12, 12], 5))
+    want = model.log_probs(ids)
+    scored, lost = runner.ops.log_probs, []
+
+    def after_the_launch(*a):
+        lost.append(True)
+        return scored(*a)
+
+    def raise_if_lost():
+        if lost:
+            lost.clear()
+            raise LostStep("void")
+    runner.ops.log_probs, runner._raise_if_lost = after_the_launch, raise_if_lost
+    model.engine.add_request(ids[0].tolist(), SamplingParams(max_new_tokens=4), "r")
+    model.engine.step()
+    with pytest.raises(LostStep):
+        model.log_probs(ids[:1])
+    # what was cached beside it is void too
+    assert not runner.cache.requests and not model.engine.has_work
+    runner.cache.check()
+    runner.ops.log_probs = scored
+    assert torch.equal(model.log_probs(ids), want)

@@ -21,6 +21,7 @@ from .config.registry import Architecture, read_config
 from .engine.batch import StepEntry
 from .engine.engine import LLMEngine
 from .engine.factory import build_runner
+from .kernels import LostStep
 from .sampling.params import SamplingParams
 from .weights.loader import Checkpoint
 
@@ -235,7 +236,7 @@ class CausalLMForSampling:
     def log_probs(self, input_ids, start_ids=None) -> torch.Tensor:
         """float32 `[batch, tokens]` on the host: the log-probability of every token under those before it in its row (0 for a row's
         first token, and for its padding): how likely the model finds a text. Rows that `forward` holds are left as they are; there
-        has to be a slot, and pages for a row, beside them."""
+        has to be a slot, and pages for a row, beside them. (`LostStep`: every row and request is forgotten.)"""
         engine = self._need_engine()
         runner = engine.runner
         rows = self._rows(input_ids, start_ids)
@@ -253,6 +254,10 @@ class CausalLMForSampling:
                     wanted = torch.tensor(toks[at + 1:at + 1 + len(part)], dtype=torch.int32).to(logits.device)
                     first = out.shape[1] - len(toks) + at + 1
                     out[b, first:first + len(part)] = runner.ops.log_probs(logits, wanted)[0].cpu()
+                    runner.raise_if_lost()            # (the numbers are here: the step has run)
+            except LostStep:
+                engine.reset()
+                raise
             finally:
                 runner.finish(key)
         return out
