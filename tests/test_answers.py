@@ -1035,3 +1035,37 @@ def test_a_score_of_a_lost_step_is_not_given(tiny_folders):
     runner.cache.check()
     runner.ops.log_probs = scored
     assert torch.equal(model.log_probs(ids), want)
+
+
+@BOTH
+def test_requests_that_allow_the_same_share_their_mask(tiny_folders, kernels):
+    """Samples of one prompt, requests with equal lists, and those at one place of a grammar."""
+    folder, cfg, _ = tiny_folders["A"]
+    vocab = cfg["vocab_size"]
+    engine = engine_of(folder, kernels, max_num_seqs=8)
+    prompts = prompts_of(vocab, [9, 12], 2)
+    seen, adjust = [], engine.runner.ops.adjust_logits
+
+    def look(logits, rules, *a):
+        seen.append(rules.flat[:8 * rules.rows].reshape(-1, 8)[:, 6].tolist())             # which of the masks each row goes by
+        return adjust(logits, rules, *a)
+    engine.runner.ops.adjust_logits = look
+    fixed = SamplingParams(max_new_tokens=6, seed=1, ignore_eos=True, allowed_tokens=list(range(5, 90)))
+    engine.add_samples(prompts[0], fixed, 4, "a")
+    engine.add_request(prompts[1], dataclasses.replace(fixed, allowed_tokens=np.arange(5, 90)), "b")
+    engine.add_request(prompts[1], dataclasses.replace(fixed, logit_bias={7: float("-inf")}), "c")
+    masks = [engine.requests[n].mask for n in ("a", ("a", 3), "b", "c")]
+    assert masks[0] is masks[1] is masks[2] and masks[3] is not masks[0]
+    engine.run()
+    assert [0, 0, 0, 0, 0, 1] in [sorted(rows) for rows in seen] and all(max(rows) <= 1 for rows in seen)
+    assert all(5 <= t < 90 for q in engine.requests.values() for t in q.output) and 7 not in engine.requests["c"].output
+    # a grammar by the length alone: all four are at the same place all the time
+    seen.clear()
+    by_length = dataclasses.replace(fixed, allowed_tokens=lambda out: range(20 * len(out), 20 * len(out) + 20))
+    names = engine.add_samples(prompts[0], by_length, 4, "d")
+    engine.run()
+    assert [0, 0, 0, 0] in seen and all([t // 20 for t in engine.requests[n].output] == list(range(6)) for n in names)
+    # one kept by nobody is not kept
+    engine.reset()
+    engine.sampler._masks_of = masks = []
+    assert not engine._masks

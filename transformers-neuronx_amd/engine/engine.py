@@ -5,6 +5,7 @@ token passes through `step()`.
 import dataclasses
 import itertools
 import time
+import weakref
 from dataclasses import dataclass
 from typing import Callable, Dict, Hashable, List, Optional, Sequence
 
@@ -57,6 +58,7 @@ class LLMEngine:
         self.sampler = Sampler(runner.ops, runner.model.device, slots=runner.cache.max_seqs, capacity=min(runner.vocab, max_len + 1),
                                last=runner.kept_tokens)
         self.requests: Dict[Hashable, Request] = {}
+        self._masks = weakref.WeakValueDictionary()       # the masks that requests go by, by their bytes
         self._ids = itertools.count()
         self._taken = 0                        # requests taken since the start or the last reset
         self.timings: List[dict] = []          # one record per step when `record_timings`
@@ -155,7 +157,7 @@ class LLMEngine:
             barred += banned_ngram_tokens(req.prompt + req.output, p.no_repeat_ngram_size)
         if barred:
             words &= ~pack_mask(vocab, [t for t in set(barred) if 0 <= t < vocab])
-        return words
+        return self._masks.setdefault(words.tobytes(), words)      # requests that allow the same share the array, and its row on the device
 
     @property
     def has_work(self) -> bool:
