@@ -458,3 +458,15 @@ def test_log_probs_of_a_long_row_are_off_by_a_few_roundings(ops):
         # and eight more for the powers, their arguments, the logarithm and the differences
         steps = 8 + -(-vocab // (16 * 512)) + 10 + 8
         assert ((got - want).abs() <= steps * 2.0 ** -24 * (1 + want.abs())).all()
+
+
+def test_what_a_copy_of_rows_says_that_it_moves(ops):
+    """As many places as the rows hold, a source once for all that it becomes."""
+    from transformers_neuronx_amd import debug
+    k, v, s = _pages([(2, 16, 8), (2, 8, 16), (7,)], torch.bfloat16, 0, 1)
+    rows = ops.row_set([k, v, s], [2, 3, None])
+    for (sources, targets, tokens), places, whole in (((([3, 3, 5], [0, 1, 2], [5, 5, 9])), 3 * 5 + 2 * 9, 5), (([3, 4], [0, 1], None), 4 * 16, 4)):
+        with debug.kernel_timer() as t:
+            ops.copy_rows(rows, sources, targets, tokens)
+        (calls, _, moved, _), = t.work_table().values()
+        assert calls == 1 and moved == places * 2 * (2 * 8) * 2 + whole * 7 * 2

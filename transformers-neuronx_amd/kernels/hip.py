@@ -2957,7 +2957,8 @@ class HipOps:
             dev = self.send_ints(np.array(words, dtype=np.int32))
         stream = _stream()
         self._call("rows", "tnx_copy_rows", rows.table.reached(stream), len(rows.tensors), host, len(words), _ptr(dev), len(groups), units,
-                   stream, work=lambda: (f"{len(groups)} to {len(pairs)} rows", (len(groups) + len(pairs)) * rows.row_bytes, 0))
+                   stream, work=lambda: (f"{len(groups)} to {len(pairs)} rows",
+                                         sum((1 + many) * rows.bytes_of(n) for _, n, _, many in groups), 0))
 
     ROW_WORDS = 256        # of a list of rows that goes along with a launch: 4 a source with its tokens, 1 a target
 

@@ -15,7 +15,8 @@ class RowSet:
     targets      the tensors that rows are copied to, of the same types and shapes but for the number of rows; left out: the
                  tensors themselves
 
-    No two of them lie in the same memory: what is copied would depend on which is copied first.
+    No two of them lie in the same memory, and none between another's first and last row: what is copied would depend on which is
+    copied first.
     """
 
     def __init__(self, tensors: Sequence[torch.Tensor], token_axes: Optional[Sequence[Optional[int]]] = None,
@@ -61,7 +62,8 @@ class RowSet:
         self.places: Optional[int] = places.pop() if places else None
         self.num_rows = min(t.shape[0] for t in self.tensors)
         self.num_target_rows = min(t.shape[0] for t in self.targets)
-        self.row_bytes = sum(w[4] * w[6] for w in words)
+        self._rows = [tuple(w[4:7]) for w in words]
+        self.row_bytes = self.bytes_of(-1)
         self._shapes = sorted({tuple(w[4:]) for w in words})
         self.words = np.array(words, dtype=np.int64)
         self.table = None                                  # the words on the device, put there by the backend
@@ -81,6 +83,10 @@ class RowSet:
         if shape[0] > 1 and strides[0] < count:
             raise ValueError("rows may not overlap")
         return x.data_ptr(), strides[0] * item, shape, item
+
+    def bytes_of(self, tokens: int) -> int:
+        """What is copied of a row that holds `tokens` tokens (below zero: all of it), in all tensors."""
+        return sum((run if tokens < 0 or inner == 0 else min(run, tokens * inner)) * outer for run, inner, outer in self._rows)
 
     def units(self, tokens: int) -> int:
         """Pieces of at most 16 bytes in what is copied of the largest row where it holds `tokens` tokens (below zero: all)."""
