@@ -470,3 +470,22 @@ def test_what_a_copy_of_rows_says_that_it_moves(ops):
             ops.copy_rows(rows, sources, targets, tokens)
         (calls, _, moved, _), = t.work_table().values()
         assert calls == 1 and moved == places * 2 * (2 * 8) * 2 + whole * 7 * 2
+
+
+@pytest.mark.parametrize("vocab", [7, 500, 20004])
+def test_the_largest_alternative_is_the_token_of_a_greedy_choice(ops, vocab):
+    """One order for both: by logit, ties to the lower id, zeros of both signs alike, NaN as -inf."""
+    inf, nan = float("inf"), float("nan")
+    g = torch.Generator(device="cuda").manual_seed(vocab)
+    x = torch.full((8, vocab), -1.0, device="cuda")
+    x[0, [2, 4]] = torch.tensor([-0.0, 0.0], device="cuda")
+    x[1, [2, 4]] = torch.tensor([0.0, -0.0], device="cuda")
+    x[2, [0, 5]] = torch.tensor([nan, 3.0], device="cuda")
+    x[3, [1, 6]] = inf
+    x[4] = nan
+    x[5] = -inf
+    x[6, 1:] = nan
+    x[7] = torch.randint(0, 3, (vocab,), generator=g, device="cuda").float()
+    ids = ops.log_probs(x, torch.zeros(8, dtype=torch.int32, device="cuda"), min(5, vocab))[1]
+    want = torch.sort(torch.where(torch.isnan(x), -inf, x), dim=1, descending=True, stable=True).indices
+    assert torch.equal(ops.argmax(x.clone()).long(), ids[:, 0].long()) and torch.equal(ids.long(), want[:, :ids.shape[1]])

@@ -9,6 +9,7 @@
 // the key; for top-p first the distance below the row's maximum), until few enough keys are left to rank in
 // LDS. The draw runs over the kept tokens in ascending order of token id.
 #include "common.h"
+#include "token_order.h"
 
 TNX_DEFINE_ERROR_API
 
@@ -16,14 +17,6 @@ TNX_DEFINE_ERROR_API
 // The most keys that are gathered in LDS and ranked against one another there (each against all: what a wave
 // reads from LDS is the limit, 256 keys take a few microseconds, 1,024 would take a hundred).
 #define SAMPLE_GATHER 256
-
-__device__ __forceinline__ uint64_t order_key(float x, int idx) {
-  if (x != x) x = -INFINITY;  // NaN orders last
-  if (x == 0.f) x = 0.f;      // -0 and +0 are one value: the lower token id decides between them
-  uint32_t u = __float_as_uint(x);
-  u = (u & 0x80000000u) ? ~u : (u | 0x80000000u);
-  return ((uint64_t)u << 32) | (uint32_t)(~(uint32_t)idx);
-}
 
 __device__ __forceinline__ float philox_uniform(uint64_t seed, uint64_t counter) {
   const uint32_t M0 = 0xD2511F53u, M1 = 0xCD9E8D57u, W0 = 0x9E3779B9u, W1 = 0xBB67AE85u;

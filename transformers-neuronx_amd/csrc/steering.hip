@@ -2,6 +2,7 @@
 // penalties for repeated tokens, biases and masks of allowed tokens (`adjust_logits`), and log-probabilities with the
 // best alternatives (`log_probs`).
 #include "common.h"
+#include "token_order.h"
 
 TNX_DEFINE_ERROR_API
 
@@ -167,20 +168,6 @@ extern "C" int tnx_adjust_logits(float* logits, const int* rules, const int* bia
 __device__ __forceinline__ float log_prob_of(float x, float m, float log_l) {
   if (!(x > -INFINITY)) return -INFINITY;          // and a NaN
   return (x == m ? 0.f : x - m) - log_l;
-}
-
-__device__ __forceinline__ unsigned long long order_key(float x, int idx) {
-  if (x != x) x = -INFINITY;
-  if (x == 0.f) x = 0.f;       // -0 and +0 are one value: the lower token id decides between them
-  unsigned u = __float_as_uint(x);
-  u = (u & 0x80000000u) ? ~u : (u | 0x80000000u);
-  return ((unsigned long long)u << 32) | (unsigned)(~(unsigned)idx);
-}
-
-// the logit of a key
-__device__ __forceinline__ float key_value(unsigned long long key) {
-  const unsigned u = (unsigned)(key >> 32);
-  return __uint_as_float((u & 0x80000000u) ? u & 0x7FFFFFFFu : ~u);
 }
 
 // log2(e) in two parts, of which the second is what the first lacks
