@@ -886,11 +886,13 @@ def test_prompts_that_waited_for_pages_go_first_once_there_are_some(tiny_folders
 
 def everything_of(m):
     """What the tables say and what the tensors hold of every request, as values to compare."""
+    def raw(t):                  # (what was never written may be no number)
+        return t.contiguous().cpu().numpy().tobytes()
     out = {}
     for req, r in m.requests.items():
         out[req] = (r.slot, r.num_tokens, {g: list(t) for g, t in r.tables.items()},
-                    [t[[p for p in r.tables[lc.group] if p >= 0]].tolist() for lc in m.caches.values() if lc.group for t in lc.pages.values()],
-                    [t[r.slot].tolist() for lc in m.caches.values() for t in lc.state.values()])
+                    [raw(t[[p for p in r.tables[lc.group] if p >= 0]]) for lc in m.caches.values() if lc.group for t in lc.pages.values()],
+                    [raw(t[r.slot]) for lc in m.caches.values() for t in lc.state.values()])
     return out, sorted(m.slots._free), {n: sorted(g.pool._free) for n, g in m.groups.items()}
 
 
