@@ -489,3 +489,23 @@ def test_the_largest_alternative_is_the_token_of_a_greedy_choice(ops, vocab):
     ids = ops.log_probs(x, torch.zeros(8, dtype=torch.int32, device="cuda"), min(5, vocab))[1]
     want = torch.sort(torch.where(torch.isnan(x), -inf, x), dim=1, descending=True, stable=True).indices
     assert torch.equal(ops.argmax(x.clone()).long(), ids[:, 0].long()) and torch.equal(ids.long(), want[:, :ids.shape[1]])
+
+
+def test_room_on_the_host_is_kept_until_all_has_arrived(ops):
+    """What was sent before and is waited for by nobody, when a larger one takes its place; and no recording writes there."""
+    small, large = torch.randn(2, 40, device="cuda"), torch.randn(1000, 40, device="cuda")
+    few, many = (ops.log_probs(x, torch.zeros(len(x), dtype=torch.int32, device="cuda"), 3) for x in (small, large))
+    ops._scores = [None, None]
+    torch.cuda.synchronize()
+    torch.cuda._sleep(100_000_000)
+    first = ops.send_log_probs(*few)
+    ops.send_log_probs(*few)
+    third = ops.send_log_probs(*many)
+    assert first[-1].query() and third[0] is not first[0]
+    assert ops.receive_log_probs(third) == tuple(t.tolist() for t in many)
+    x = torch.zeros(4, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(RuntimeError, match="recorded"):
+            ops.send_log_probs(*few)
+        x.add_(1)

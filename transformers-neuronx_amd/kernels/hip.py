@@ -546,6 +546,20 @@ class _Sent:
         return self.at
 
 
+class _Room:
+    """Pinned host memory that a kernel writes what is on its way to the host, and the event after the last that did."""
+
+    __slots__ = ("host", "address", "landed")
+
+    def __init__(self, host: torch.Tensor, address):
+        self.host, self.address, self.landed = host, address, None
+
+    def sent(self) -> "torch.cuda.Event":
+        self.landed = torch.cuda.Event()
+        self.landed.record()
+        return self.landed
+
+
 class HipOps:
     name = "hip"
 
@@ -672,13 +686,19 @@ class HipOps:
         pinned host memory by the same kernel. Returns what `receive_tokens` takes."""
         n = tokens.numel()
         self._landing_turn ^= 1
-        pinned = self._landing[self._landing_turn]
-        if pinned is None or pinned[0].numel() < n:
-            pinned = self._landing[self._landing_turn] = self.pinned_ints(max(2 * n, 256))
-        self.store_tokens(kept, tokens, ctx, pinned[1])
-        landed = torch.cuda.Event()
-        landed.record()
-        return pinned[0], n, landed
+        room = self._room(self._landing, self._landing_turn, n)
+        self.store_tokens(kept, tokens, ctx, room.address)
+        return room.host, n, room.sent()
+
+    def _room(self, rooms, turn, n) -> "_Room":
+        """Pinned memory for `n` integers on their way to the host. One that is too small goes only when what was sent there has arrived,
+        also where nobody waits for it any more: freed memory may be another's at once."""
+        room = rooms[turn]
+        if room is None or room.host.numel() < n:
+            if room is not None and room.landed is not None:
+                room.landed.synchronize()
+            room = rooms[turn] = _Room(*self.pinned_ints(max(2 * n, 256)))
+        return room
 
     def receive_tokens(self, sent):
         host, n, landed = sent
@@ -3088,15 +3108,15 @@ class HipOps:
         if top:
             _want(ids, "tokens", torch.int32, (rows, top))
             _want(best, "their log-probabilities", torch.float32, (rows, top))
-        n = rows * (1 + 2 * top)
+        self._on_this_device(out.device, "log-probabilities")
+        if top and not out.device == ids.device == best.device:
+            raise ValueError("log-probabilities and the alternatives lie on different devices")
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("send_log_probs writes to the host's memory in turn and cannot be recorded into a graph")
         self._scores_turn ^= 1
-        pinned = self._scores[self._scores_turn]
-        if pinned is None or pinned[0].numel() < n:
-            pinned = self._scores[self._scores_turn] = self.pinned_ints(max(2 * n, 256))
-        self._call("steering", "tnx_send_log_probs", _ptr(out), _ptr(best), _ptr(ids), rows, top, pinned[1], _stream())
-        landed = torch.cuda.Event()
-        landed.record()
-        return pinned[0], rows, top, landed
+        room = self._room(self._scores, self._scores_turn, rows * (1 + 2 * top))
+        self._call("steering", "tnx_send_log_probs", _ptr(out), _ptr(best), _ptr(ids), rows, top, room.address, _stream())
+        return room.host, rows, top, room.sent()
 
     def receive_log_probs(self, sent):
         host, rows, top, landed = sent
