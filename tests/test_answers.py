@@ -1071,3 +1071,31 @@ def test_requests_that_allow_the_same_share_their_mask(tiny_folders, kernels):
     engine.reset()
     engine.sampler._masks_of = masks = []
     assert not engine._masks
+
+
+@pytest.mark.parametrize("call", ["resize", "reorder", "fork", "score"])
+def test_a_lost_step_found_between_two_steps_forgets_every_request(tiny_folders, call):
+    """Also where it is found by a call that runs no step of the engine's: nothing goes on from a cache that is void."""
+    from transformers_neuronx_amd import ContinuousBatchingConfig, NeuronConfig
+    from transformers_neuronx_amd.kernels import LostStep
+    folder, cfg, _ = tiny_folders["A"]
+    model = model_of(folder, "reference", neuron_config=NeuronConfig(continuous_batching=ContinuousBatchingConfig(max_num_seqs=4)))
+    engine, ids = model.engine, torch.tensor(prompts_of(cfg["vocab_size"], [12], 5))
+    model.forward(ids)
+    model.forward(ids, cache_ids=torch.arange(12).unsqueeze(0), start_ids=[1])
+    params = SamplingParams(max_new_tokens=6, do_sample=False, ignore_eos=True)
+    engine.add_request(ids[0].tolist(), params, "r")
+    for _ in range(3):
+        engine.step()
+    asked = engine.runner._raise_if_lost
+
+    def lost():
+        engine.runner._raise_if_lost = asked
+        raise LostStep("void")
+    engine.runner._raise_if_lost = lost
+    with pytest.raises(LostStep):
+        {"resize": lambda: engine.resize_cache(30), "reorder": lambda: model.reorder_cache([0, 0]),
+         "fork": lambda: model.fork_sequence(1, 2), "score": lambda: model.log_probs(ids)}[call]()
+    assert not engine.has_work and not engine.requests and not engine.runner.cache.requests
+    engine.runner.cache.check()
+    assert engine.generate([ids[0].tolist()], params) == model_of(folder, "reference").engine.generate([ids[0].tolist()], params)

@@ -21,7 +21,6 @@ from .config.registry import Architecture, read_config
 from .engine.batch import StepEntry
 from .engine.engine import LLMEngine
 from .engine.factory import build_runner
-from .kernels import LostStep
 from .sampling.params import SamplingParams
 from .weights.loader import Checkpoint
 
@@ -221,16 +220,18 @@ class CausalLMForSampling:
         rows of a parent share its full pages, and only the page that is not full, and the fixed state, are copied. The rows are those
         of the last `forward` that began a batch; more of them may be asked for, up to the model's batch size: a search begins with
         one row of the prompt, which becomes as many as it has beams."""
-        runner = self._need_engine().runner
+        engine = self._need_engine()
         parents = [int(p) for p in torch.as_tensor(beam_idx).flatten()]
-        runner.reorder([("row", b) for b in range(len(parents))], parents)
+        with engine.forgets_if_lost():
+            engine.runner.reorder([("row", b) for b in range(len(parents))], parents)
 
     def fork_sequence(self, seq_id: int, new_seq_id: int) -> None:
         """Sequence `new_seq_id` of the continuous-batching form goes on from what `seq_id` holds; one that it held before is over."""
-        runner = self._need_engine().runner
-        if int(seq_id) == int(new_seq_id) or not runner.cache.has(("seq", int(seq_id))):
+        engine = self._need_engine()
+        if int(seq_id) == int(new_seq_id) or not engine.runner.cache.has(("seq", int(seq_id))):
             raise ValueError(f"sequence {seq_id} holds nothing that sequence {new_seq_id} could go on from")
-        runner.reorder([("seq", int(seq_id)), ("seq", int(new_seq_id))], [0, 0])
+        with engine.forgets_if_lost():
+            engine.runner.reorder([("seq", int(seq_id)), ("seq", int(new_seq_id))], [0, 0])
 
     @torch.no_grad()
     def log_probs(self, input_ids, start_ids=None) -> torch.Tensor:
@@ -250,14 +251,12 @@ class CausalLMForSampling:
             try:
                 for at in range(0, len(toks) - 1, portion):
                     part = toks[at:min(at + portion, len(toks) - 1)]
-                    logits = runner.step([StepEntry(key, part, list(range(len(part))))])
-                    wanted = torch.tensor(toks[at + 1:at + 1 + len(part)], dtype=torch.int32).to(logits.device)
-                    first = out.shape[1] - len(toks) + at + 1
-                    out[b, first:first + len(part)] = runner.ops.log_probs(logits, wanted)[0].cpu()
-                    runner.raise_if_lost()            # (the numbers are here: the step has run)
-            except LostStep:
-                engine.reset()
-                raise
+                    with engine.forgets_if_lost():
+                        logits = runner.step([StepEntry(key, part, list(range(len(part))))])
+                        wanted = torch.tensor(toks[at + 1:at + 1 + len(part)], dtype=torch.int32).to(logits.device)
+                        first = out.shape[1] - len(toks) + at + 1
+                        out[b, first:first + len(part)] = runner.ops.log_probs(logits, wanted)[0].cpu()
+                        runner.raise_if_lost()            # (the numbers are here: the step has run)
             finally:
                 runner.finish(key)
         return out

@@ -2,6 +2,7 @@
 function and the sampler; everything between a request's tokens and its next
 token passes through `step()`.
 """
+import contextlib
 import dataclasses
 import itertools
 import time
@@ -142,7 +143,8 @@ class LLMEngine:
 
     def resize_cache(self, num_pages) -> None:
         """Another number of cache pages, between two steps; live requests keep theirs (`ModelRunner.resize_cache`)."""
-        self.runner.resize_cache(num_pages)
+        with self.forgets_if_lost():
+            self.runner.resize_cache(num_pages)
         self.scheduler.pool_resized()
 
     def _mask(self, req: Request):
@@ -269,6 +271,15 @@ class LLMEngine:
         the tokens under way, and the keys and values cached with them, are void, and every request is forgotten."""
         try:
             return self._step()
+        except LostStep:
+            self.reset()
+            raise
+
+    @contextlib.contextmanager
+    def forgets_if_lost(self):
+        """Where what has run is found void, every request is forgotten with what is cached of it: for calls between two steps."""
+        try:
+            yield
         except LostStep:
             self.reset()
             raise
