@@ -1041,7 +1041,7 @@ def test_a_score_of_a_lost_step_is_not_given(tiny_folders):
 
 @BOTH
 def test_requests_that_allow_the_same_share_their_mask(tiny_folders, kernels):
-    """Samples of one prompt, requests with equal lists, and those at one place of a grammar."""
+    """Samples of one prompt, and requests with equal lists."""
     folder, cfg, _ = tiny_folders["A"]
     vocab = cfg["vocab_size"]
     engine = engine_of(folder, kernels, max_num_seqs=8)
@@ -1061,12 +1061,6 @@ def test_requests_that_allow_the_same_share_their_mask(tiny_folders, kernels):
     engine.run()
     assert [0, 0, 0, 0, 0, 1] in [sorted(rows) for rows in seen] and all(max(rows) <= 1 for rows in seen)
     assert all(5 <= t < 90 for q in engine.requests.values() for t in q.output) and 7 not in engine.requests["c"].output
-    # a grammar by the length alone: all four are at the same place all the time
-    seen.clear()
-    by_length = dataclasses.replace(fixed, allowed_tokens=lambda out: range(20 * len(out), 20 * len(out) + 20))
-    names = engine.add_samples(prompts[0], by_length, 4, "d")
-    engine.run()
-    assert [0, 0, 0, 0] in seen and all([t // 20 for t in engine.requests[n].output] == list(range(6)) for n in names)
     # one kept by nobody is not kept
     engine.reset()
     engine.sampler._masks_of = masks = []

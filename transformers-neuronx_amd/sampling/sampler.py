@@ -66,7 +66,7 @@ class Sampler:
             history = self._history = self.ops.token_history(self.slots, self.capacity)
         if starts:
             self.ops.start_history(history, [s.slot for s in starts], [s.start[0] for s in starts], [s.start[1] for s in starts], self.last)
-        # rows of one grammar, at the same place in it, share their mask
+        # rows whose masks are one array share it (requests with equal lists of allowed tokens)
         arrays: List[np.ndarray] = []
         mask_rows = []
         for s in rows:
