@@ -1093,3 +1093,58 @@ def test_a_lost_step_found_between_two_steps_forgets_every_request(tiny_folders,
     assert not engine.has_work and not engine.requests and not engine.runner.cache.requests
     engine.runner.cache.check()
     assert engine.generate([ids[0].tolist()], params) == model_of(folder, "reference").engine.generate([ids[0].tolist()], params)
+
+
+@BOTH
+@pytest.mark.parametrize("state", [False, True])
+def test_reorders_at_random_with_hardly_any_room(kernels, state):
+    """Beams that grow, change places and become more or fewer, in pools where the pages and slots of those that are over are needed at once:
+    done and right, or refused and unchanged."""
+    rng = random.Random(7)
+    done = refused = 0
+    for trial in range(12):
+        m = manager(kernels, state=state, num_pages=rng.choice([14, 18, 26]), max_seqs=rng.choice([4, 5, 6]))
+        texts, states = {}, {}
+        m.add_request("other")                                    # one that takes no part, and shares nothing
+        m.grow("other", 9)
+        fill(m, "other", 0, list(range(1, 10)))
+        m.advance("other", 9)
+        m.add_request(0)
+        texts[0], states[0] = [], 0.0
+        for turn in range(25):
+            n = rng.choice([1, 1, 3, 15, 16])
+            for name in sorted(texts):
+                if m.can_grow(name, len(texts[name]) + n) and len(texts[name]) < 70:
+                    values = [rng.randrange(1, 1 << 12) for _ in range(n)]
+                    m.grow(name, len(texts[name]) + n)
+                    fill(m, name, len(texts[name]), values)
+                    m.advance(name, n)
+                    texts[name] = texts[name] + values
+                states[name] = rng.randrange(1 << 12)
+                for t in m.caches[3].state.values() if state else ():
+                    t[m.slot_of(name)] = states[name]
+            width = rng.randint(1, 5)
+            parents = [rng.choice(sorted(texts)) for _ in range(width)]
+            before = everything_of(m) if kernels == "reference" else None
+            try:
+                m.reorder(list(range(width)), parents)
+            except (OutOfPages, OutOfSlots, ValueError):
+                refused += 1
+                assert before is None or everything_of(m) == before
+            else:
+                done += 1
+                kept = {b: texts[b] for b in texts if b >= width}
+                kept_states = {b: states[b] for b in kept}
+                texts = {**kept, **{b: texts[p] for b, p in enumerate(parents)}}
+                states = {**kept_states, **{b: states[p] for b, p in enumerate(parents)}}
+            m.check()
+            assert set(m.requests) == set(texts) | {"other"} and m.slots.num_free == m.max_seqs - len(m.requests)
+            holds(m, "other", list(range(1, 10)))
+            for name in texts:
+                holds(m, name, texts[name])
+                assert not state or all((t[m.slot_of(name)] == states[name]).all() for t in m.caches[3].state.values())
+            if rng.random() < 0.3 and len(texts) > 1:
+                name = rng.choice(sorted(texts))
+                m.free_request(name)
+                del texts[name], states[name]
+    assert done > 100 and refused > 10
