@@ -1148,3 +1148,17 @@ def test_reorders_at_random_with_hardly_any_room(kernels, state):
                 m.free_request(name)
                 del texts[name], states[name]
     assert done > 100 and refused > 10
+
+
+def test_samples_of_the_last_seed_there_is(tiny_folders):
+    """Seeds are 64 bits: the one behind the last is the first."""
+    folder, cfg, _ = tiny_folders["A"]
+    prompt = prompts_of(cfg["vocab_size"], [8], 3)[0]
+    params = SamplingParams(max_new_tokens=12, temperature=1.5, seed=2 ** 63 - 2, ignore_eos=True)
+    engine = engine_of(folder, "reference")
+    names = engine.add_samples(prompt, params, 4)
+    engine.run()
+    assert [engine.requests[n].params.seed for n in names] == [2 ** 63 - 2, 2 ** 63 - 1, -2 ** 63, -2 ** 63 + 1]
+    assert len({tuple(engine.requests[n].output) for n in names}) == 4
+    model = model_of(folder, "reference")
+    assert model.sample(torch.tensor([prompt, prompt]), 14, seed=2 ** 63 - 2, num_return_sequences=2).shape == (4, 14)

@@ -21,6 +21,7 @@ from .config.registry import Architecture, read_config
 from .engine.batch import StepEntry
 from .engine.engine import LLMEngine
 from .engine.factory import build_runner
+from .engine.scheduler import seed_behind
 from .sampling.params import SamplingParams
 from .weights.loader import Checkpoint
 
@@ -312,13 +313,13 @@ class CausalLMForSampling:
                 if gen.global_top_k is not None:
                     k = min(k, int(gen.global_top_k)) if k > 0 else int(gen.global_top_k)
                 p = SamplingParams(max_new_tokens=new, do_sample=gen.do_sample, temperature=float(line(gen.temperature)),
-                                   top_k=k, top_p=float(line(gen.top_p)), seed=seed + b * made,
+                                   top_k=k, top_p=float(line(gen.top_p)), seed=seed_behind(seed, b * made),
                                    min_tokens_to_keep=int(line(gen.top_p_min_tokens)), deterministic=gen.deterministic,
                                    eos_token_id=gen.eos_token_id, ignore_eos=gen.eos_token_id is None,
                                    no_repeat_ngram_size=int(no_repeat_ngram_size or 0), **steered)
             else:
                 p = SamplingParams(max_new_tokens=new, do_sample=True, temperature=temperature, top_k=top_k,
-                                   top_p=top_p, seed=seed + b * made,
+                                   top_p=top_p, seed=seed_behind(seed, b * made),
                                    eos_token_id=(eos_token_id if eos_token_id is not None
                                                  else getattr(self.config, 'eos_token_id', None)),
                                    ban_eos=True, ignore_eos=True, no_repeat_ngram_size=int(no_repeat_ngram_size or 0), **steered)

@@ -19,7 +19,7 @@ from ..kernels.steering import pack_mask
 from ..sampling.sampler import Sampler, Steering, banned_ngram_tokens
 from .batch import StepEntry
 from .runner import ModelRunner
-from .scheduler import PENDING, Family, Request, ScheduledRun, Scheduler
+from .scheduler import PENDING, Family, Request, ScheduledRun, Scheduler, seed_behind
 
 
 @dataclass
@@ -118,7 +118,8 @@ class LLMEngine:
         for name in names:
             if name in self.requests and not self.requests[name].finished:
                 raise ValueError(f"request {name!r} is already live")
-        streams = [params] + [params if params.seed is None else dataclasses.replace(params, seed=params.seed + i) for i in range(1, count)]
+        streams = [params] + [params if params.seed is None else dataclasses.replace(params, seed=seed_behind(params.seed, i))
+                               for i in range(1, count)]
         for i, (name, stream) in enumerate(zip(names, streams)):
             try:
                 self._add(prompt, stream, name, leader=self.requests[names[0]] if i else None)

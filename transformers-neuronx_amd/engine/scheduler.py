@@ -41,6 +41,11 @@ from ..sampling.params import SamplingParams
 PENDING = -1              # stands in `Request.output` for a token that is drawn but not read yet
 
 
+def seed_behind(seed: int, count: int) -> int:
+    """The seed that lies `count` behind another: 64 bits with a sign, the first behind the last."""
+    return (int(seed) + count + 2 ** 63) % 2 ** 64 - 2 ** 63
+
+
 @dataclass
 class Family:
     """A request and all that were forked from it, and from those: no two of them draw from one random stream unless they are told to."""
@@ -50,7 +55,7 @@ class Family:
     def next_seed(self) -> int:
         """A seed that no other of the family has, nor the samples of a prompt beside it, whose seeds follow one another."""
         self.forks += 1
-        return (self.seed + (self.forks << 40) + 2 ** 63) % 2 ** 64 - 2 ** 63
+        return seed_behind(self.seed, self.forks << 40)
 
 
 @dataclass(eq=False)      # a request is itself: lists of requests are searched by identity
