@@ -150,3 +150,12 @@ def test_a_full_history_and_tokens_of_no_vocabulary_on_the_host():
     rules = OPS.logit_rules(4, slots=[0, 1], presence=[0.5, 0.5])
     OPS.adjust_logits(logits, rules, history, torch.tensor([3, 99], dtype=torch.int32))
     assert logits.tolist() == [[0.5, 0.5, 1, 1], [1, 1, 1, 1]] and torch.equal(history.entries, entries) and history.used.tolist() == [2, 2]
+
+
+@pytest.mark.parametrize("bad", [2 ** 32 + 5, 2 ** 31, -2 ** 31 - 1, -1])
+def test_tokens_that_are_no_32_bits_begin_no_history(bad):
+    """They would be entered as other tokens."""
+    for prompt, output in (([1, bad], []), ([1], [bad])):
+        with pytest.raises(ValueError, match="token"):
+            TokenHistory.distinct(prompt, output)
+    assert TokenHistory.distinct([2 ** 31 - 1], [0]).tolist() == [[2 ** 31 - 1, 1], [0, 2]]

@@ -3002,8 +3002,6 @@ class HipOps:
         longest = max(len(e) for e in lists)
         if longest > history.capacity:
             raise ValueError(f"a sequence of {longest} distinct tokens, the history holds {history.capacity}")
-        if any(len(e) and e[:, 0].min() < 0 for e in lists):
-            raise ValueError("a token is below zero")
         self._on_this_device(history.entries.device, "history")
         if last is not None:
             _want(last, "last", torch.int32)

@@ -31,6 +31,8 @@ class TokenHistory:
         if tokens.size == 0:
             return np.zeros((0, 2), dtype=np.int32)
         ids, first, which = np.unique(tokens, return_index=True, return_inverse=True)
+        if ids[0] < 0 or ids[-1] >= 2 ** 31:
+            raise ValueError(f"a token is a number from 0 to 2^31 - 1, got {int(ids[0] if ids[0] < 0 else ids[-1])}")
         times = np.bincount(which.reshape(-1)[split:], minlength=len(ids))
         order = np.argsort(first)
         out = np.empty((len(ids), 2), dtype=np.int32)
