@@ -1162,3 +1162,18 @@ def test_samples_of_the_last_seed_there_is(tiny_folders):
     assert len({tuple(engine.requests[n].output) for n in names}) == 4
     model = model_of(folder, "reference")
     assert model.sample(torch.tensor([prompt, prompt]), 14, seed=2 ** 63 - 2, num_return_sequences=2).shape == (4, 14)
+
+
+def test_biases_are_those_at_the_beginning(tiny_folders):
+    """A dictionary that its owner goes on to change steers neither a request made before nor what is made of its params."""
+    folder, cfg, _ = tiny_folders["A"]
+    biases = {40: 1000.0}
+    params = SamplingParams(max_new_tokens=4, seed=5, ignore_eos=True, logit_bias=biases)
+    biases[41] = 2000.0
+    engine = engine_of(folder, "reference")
+    names = engine.add_samples([3, 4, 5], params, 3)
+    names.append(engine.fork_request(names[0]))
+    names.append(engine.add_request([3, 4, 5], dataclasses.replace(params, seed=None)))
+    engine.run()
+    assert all(engine.requests[n].output == [40] * 4 for n in names)
+    assert params.logit_bias == {40: 1000.0} and SamplingParams().logit_bias is None

@@ -80,6 +80,8 @@ class SamplingParams:
         biases = {operator.index(t): float(b) for t, b in dict(self.logit_bias or {}).items()}
         if any(not (abs(b) <= most or b == float("-inf")) for b in biases.values()):
             raise ValueError("a logit bias is a finite number, or -inf for a token that must not be chosen")
+        if self.logit_bias is not None:
+            self.logit_bias = biases                     # not the caller's, who may go on to change it
         self.biases: Tuple[Tuple[int, float], ...] = tuple(sorted(biases.items()))     # what is gone by from here on
         if self.logprobs is not None and not (isinstance(self.logprobs, int) and 0 <= self.logprobs <= self.MOST_LOGPROBS):
             raise ValueError(f"logprobs has to be an integer from 0 to {self.MOST_LOGPROBS}, but is {self.logprobs}")
